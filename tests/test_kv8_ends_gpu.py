@@ -1,0 +1,23 @@
+"""The 8-bit caches' attention at the ends of its range, against the definition in 64 bits: weights that nearly cancel, zero
+queries over zero keys, scores past 2^24, scores of minus infinity, value scales far apart."""
+
+import pytest
+import torch
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA GPU")]
+
+from test_kv8_gpu import DTYPES, _attend, _check, _check_cross, _cross_reference, _gen, _randn, _self_case, _values  # noqa: E402
+from whisper_trt_b200 import kv8  # noqa: E402
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("s,t", [(5, 2), (8, 6), (16, 2), (24, 6), (32, 2), (40, 2), (70, 6), (130, 2)])
+def test_cross_weights_in_two_parts(dtype, s, t):
+    """Frames in pairs of opposite values and nearly equal weights: what is left of a pair shows the weights' own bits. Scores
+    of about 2^-6, so that their fp32 sums are no part of the error; weights in two parts of 11 bits err by 2^-22."""
+    g = _gen(s + t)
+    k, v = _randn(g, 30, 4, t, 64, dtype=dtype), _randn(g, 30, 4, t, 64, dtype=dtype)
+    v[:, :, 1::2] = -v[:, :, ::2]
+    cache = kv8.quantize_cross(k, v)
+    q = _randn(g, 30, s, 256, std=2.0**-7, dtype=dtype)
+    _check(kv8.cross_attn(q, cache), *_cross_reference(q, cache, None), 2.0**-22)

@@ -205,21 +205,18 @@ __device__ __forceinline__ void unit_values(uint32_t (&va)[2][4][4], const unsig
     }
   }
 }
-// One tile's weights (in unit_scores' order) as fp16, or hi + lo parts of it, into the output.
-template <bool SPLIT>
+// One tile's weights (in unit_scores' order) as hi + lo parts in fp16 into the output.
 __device__ __forceinline__ void unit_output(float (&o)[4][4], const uint32_t (&va)[4][4], float p0, float p1, float p2,
                                             float p3) {
   const uint32_t h01 = Elem<__half>::from_float2(p0, p1), h23 = Elem<__half>::from_float2(p2, p3);
   const uint32_t pb0 = movmatrix(h01), pb1 = movmatrix(h23);
 #pragma unroll
   for (int i = 0; i < 4; ++i) mma_f16(o[i], va[i][0], va[i][1], va[i][2], va[i][3], pb0, pb1);
-  if (SPLIT) {
-    const float2 f01 = Elem<__half>::to_float2(h01), f23 = Elem<__half>::to_float2(h23);
-    const uint32_t lb0 = movmatrix(Elem<__half>::from_float2(p0 - f01.x, p1 - f01.y));
-    const uint32_t lb1 = movmatrix(Elem<__half>::from_float2(p2 - f23.x, p3 - f23.y));
+  const float2 f01 = Elem<__half>::to_float2(h01), f23 = Elem<__half>::to_float2(h23);
+  const uint32_t lb0 = movmatrix(Elem<__half>::from_float2(p0 - f01.x, p1 - f01.y));
+  const uint32_t lb1 = movmatrix(Elem<__half>::from_float2(p2 - f23.x, p3 - f23.y));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mma_f16(o[i], va[i][0], va[i][1], va[i][2], va[i][3], lb0, lb1);
-  }
+  for (int i = 0; i < 4; ++i) mma_f16(o[i], va[i][0], va[i][1], va[i][2], va[i][3], lb0, lb1);
 }
 
 }  // namespace wt

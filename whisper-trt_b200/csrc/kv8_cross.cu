@@ -12,8 +12,8 @@
 // The products run on mma.sync with keys as rows: S^T = K Q^T, O^T += V^T P^T, 16 keys by 8 queries. e4m3 converts to
 // fp16 exactly, so the operands are the stored values and the fp16 queries (query_exp: bf16 ones scaled), and the scales
 // are applied to the fp32 results: the scores times k_scale and the query's power, a unit's output times v_scale as
-// it is added. The weights enter as fp16; for fp16 outputs as two parts, hi + lo, so that their rounding (2^-12 each,
-// the output's own half step) does not add to the output's; for bf16 outputs one part errs by an eighth of theirs.
+// it is added. The weights enter as fp16 in two parts, hi + lo (22 significant bits): one part alone errs by 2^-12 of the
+// sum of p |v|, which shows in any output that is small beside it, bf16 ones too.
 // How the operands come to lie in registers: unit_scores and unit_values in kv8.cuh.
 #include <cooperative_groups.h>
 
@@ -31,7 +31,6 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
                   const float *__restrict__ ks, const float *__restrict__ vs, const int64_t *__restrict__ lengths,
                   T *__restrict__ y, int S, int H, int Tn, int nblk, int cl, float scale) {
   namespace cg = cooperative_groups;
-  constexpr bool kSplit = Elem<T>::code != WT_BF16;
   constexpr int kRing = STAGES * kUnitBytes;
   static_assert(NT * 8 * kRec * 4 <= kRing, "a warp's records lie over its ring");
   extern __shared__ __align__(128) unsigned char smem[];
@@ -198,7 +197,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
         const float p2 = ex2f(sc[nt][t][2] + up0), p3 = ex2f(sc[nt][t][3] + up1);
         s0 += p0 + p2;
         s1 += p1 + p3;
-        unit_output<kSplit>(tmp, va[t], p0, p1, p2, p3);
+        unit_output(tmp, va[t], p0, p1, p2, p3);
       }
       l[nt][0] = fmaf(s0, kWeightInv, l[nt][0]);
       l[nt][1] = fmaf(s1, kWeightInv, l[nt][1]);

@@ -30,7 +30,6 @@ __global__ void __launch_bounds__(kSWarps * 32, kSResident / kSWarps)
                       const float *__restrict__ ks, const float *__restrict__ vs, const int64_t *__restrict__ offset,
                       const int32_t *__restrict__ src, T *__restrict__ y, int N, int H, int C, int cl, float scale) {
   namespace cg = cooperative_groups;
-  constexpr bool kSplit = true;
   __shared__ __align__(128) unsigned char smem[kSWarps * kSRing];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
@@ -196,7 +195,7 @@ __global__ void __launch_bounds__(kSWarps * 32, kSResident / kSWarps)
       sum += p0 + p1;
       p0 *= w[t][0] * inv;
       p1 *= w[t][1] * inv;
-      unit_output<kSplit>(tmp, va[t], p0, p0, p1, p1);
+      unit_output(tmp, va[t], p0, p0, p1, p1);
     }
     l = fmaf(sum, kWeightInv, l);
     const float by = big * kWeightInv;

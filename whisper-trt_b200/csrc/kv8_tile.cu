@@ -23,8 +23,7 @@
 // Scales: a score is multiplied by the block's key scale and the query's power (query_exp), a weight by the block's
 // value scale over a reference, the largest one so far, by whose change the output is rescaled like a maximum's. Weights enter
 // as fp16, 2^kUp times themselves (at most 2^15), normal down to 2^-(14 + kUp) of the reference maximum and never off by
-// more than 2^-(25 + kUp) of it; for fp16 outputs as two parts, hi + lo, so that their rounding does not add to the
-// output's. Waits are bounded as in the other tcgen05 kernels: a wait that runs out sets the error word and a stop flag.
+// more than 2^-(25 + kUp) of it, in two parts, hi + lo, so that their rounding does not add to the output's. Waits are bounded as in the other tcgen05 kernels: a wait that runs out sets the error word and a stop flag.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
@@ -120,7 +119,6 @@ template <typename T, bool SHARED>
 __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
   namespace cg = cooperative_groups;
   const int cl = SHARED ? a.cl : 1;
-  constexpr bool kLo = Elem<T>::code != WT_BF16;  // weights in two parts
   constexpr int kStages = kTStages;
   extern __shared__ unsigned char smem_raw[];
   unsigned char *smem =
@@ -302,7 +300,7 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       const float up[2] = {kUp - (m[0] == kNegInf ? 0.f : m[0]) + static_cast<float>(re),
                            kUp - (m[1] == kNegInf ? 0.f : m[1]) + static_cast<float>(re)};
       const Pair f2[2] = {pair_of(f[0], f[0]), pair_of(f[1], f[1])}, up2[2] = {pair_of(up[0], up[0]), pair_of(up[1], up[1])};
-      uint32_t hi[16], lo[kLo ? 16 : 1];
+      uint32_t hi[16], lo[16];
       Pair sum[2] = {0, 0};
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -314,14 +312,12 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
         const Pair p = pair_of(p0, p1);
         sum[e] = add2(sum[e], p);
         hi[j] = Elem<__half>::from_float2(p0, p1);
-        if (kLo) {
-          const float2 r = Elem<__half>::to_float2(hi[j]);
-          halves(add2(p, pair_of(-r.x, -r.y)), p0, p1);
-          lo[kLo ? j : 0] = Elem<__half>::from_float2(p0, p1);
-        }
+        const float2 r = Elem<__half>::to_float2(hi[j]);
+        halves(add2(p, pair_of(-r.x, -r.y)), p0, p1);
+        lo[j] = Elem<__half>::from_float2(p0, p1);
       }
       tmem_st_pairs(at, hi);
-      if constexpr (kLo) tmem_st_pairs(at + 32, lo);
+      tmem_st_pairs(at + 32, lo);
       const float down = exp2_int(-re);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -442,7 +438,7 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       const uint64_t vd = kvd + ((i % kStages) * 2 + 1) * (kTKTile >> 4);
       const uint32_t pa = tmem + static_cast<uint32_t>(i % kTScores * kTK);
 #pragma unroll
-      for (int s = 0; s < (kLo ? 8 : 4); ++s)  // (the second parts stand behind the first)
+      for (int s = 0; s < 8; ++s)  // (the second parts stand behind the first)
         umma_f16_ta(tmem_o, pa + 8 * s, vd + (2048 >> 4) * (s & 3), idesc_v, i > 0 || s > 0);
       umma_commit(&kv_empty[i % kStages]);
       umma_commit(&pv_done[i % kTScores]);
