@@ -21,3 +21,22 @@ def test_cross_weights_in_two_parts(dtype, s, t):
     cache = kv8.quantize_cross(k, v)
     q = _randn(g, 30, s, 256, std=2.0**-7, dtype=dtype)
     _check(kv8.cross_attn(q, cache), *_cross_reference(q, cache, None), 2.0**-22)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("s", [5, 40, 130])
+@pytest.mark.parametrize("w,t", [(20, 100), (1, 100), (1, 1500)])
+def test_cross_zero_queries_over_zero_keys(dtype, s, w, t):
+    """Zero rows and a last, partly filled block of zero keys (a padded transcript over a padded window): their scores are 0,
+    whatever the product of the two scales is in fp32. Tiny ones alike."""
+    g = _gen(s + t)
+    k, v = _randn(g, w, 2, t, 64, dtype=dtype), _randn(g, w, 2, t, 64, dtype=dtype)
+    k[:, :, t // 64 * 64:] = 0
+    q = _randn(g, w, s, 128, dtype=dtype)
+    q[:, ::3] = 0
+    q[:, 1::3] *= 2.0**-100 if dtype == torch.bfloat16 else 2.0**-20
+    y = _check_cross(q, kv8.quantize_cross(k, v))
+    assert torch.isfinite(y).all()
+    zero = kv8.quantize_cross(torch.zeros_like(k), v)
+    _check_cross(torch.zeros_like(q), zero)
+    _check_cross(torch.zeros_like(q), zero, torch.full((w,), t - 1, device="cuda"))

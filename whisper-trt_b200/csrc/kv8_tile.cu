@@ -230,7 +230,9 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
     const float factor[2] = {ok ? q_fac[row0 + (lane >> 2)] : 0.f, ok ? q_fac[row0 + (lane >> 2) + 8] : 0.f};
     for (int i = 0; i < nb && ok; ++i) {
       const uint32_t at = tmem + rows + static_cast<uint32_t>(i % kTScores * kTK);
-      const float f[2] = {next_k * factor[0], next_k * factor[1]}, top = next_v;
+      // (held above 0, where zero or tiny queries meet zero or tiny keys: frames that are not there are -inf before it)
+      constexpr float kLeast = 1.17549435e-38f;
+      const float f[2] = {fmaxf(next_k * factor[0], kLeast), fmaxf(next_k * factor[1], kLeast)}, top = next_v;
       if (i + 1 < nb) {
         next_k = a.ks[sbase + i + 1];
         next_v = a.vs[sbase + i + 1];
