@@ -40,3 +40,57 @@ def test_cross_zero_queries_over_zero_keys(dtype, s, w, t):
     zero = kv8.quantize_cross(torch.zeros_like(k), v)
     _check_cross(torch.zeros_like(q), zero)
     _check_cross(torch.zeros_like(q), zero, torch.full((w,), t - 1, device="cuda"))
+
+
+# A score of 8 a b (natural units) at the frames that count, all of them equal, and far below it at the others.
+_LARGE = [(torch.float16, 2000.0, 1024.0), (torch.float16, 2000.0, 2048.0), (torch.float16, 60000.0, 28672.0),
+          (torch.float16, 2000.0, -1024.0), (torch.float16, 60000.0, -14336.0), (torch.bfloat16, 1024.0, 2048.0),
+          (torch.bfloat16, 2.0**20, 2.0**23), (torch.bfloat16, 2.0**40, -2.0**60), (torch.bfloat16, 1920.0, -2048.0)]
+
+
+def _others(b):
+    return -b if b > 0 else 2 * b
+
+
+@pytest.mark.parametrize("dtype,a,b", _LARGE)
+@pytest.mark.parametrize("w,s,t", [(20, 5, 150), (1, 16, 300), (20, 32, 150), (20, 40, 150), (1, 70, 700)])
+def test_cross_scores_past_2_24(dtype, a, b, w, s, t):
+    """Scores whose unit in the last place is 1 or more: the softmax subtracts its maximum, and equal scores stay equal, so
+    the output is the mean over the frames that have it (no error of scores enters)."""
+    g = _gen(s + t)
+    k = torch.full((w, 1, t, 64), b, device="cuda")
+    k[:, :, torch.rand(t, generator=g, device="cuda") < 0.6] = _others(b)
+    k[:, :, [3, -1]] = b
+    cache = kv8.quantize_cross(k.to(dtype), _randn(g, w, 1, t, 64, dtype=dtype))
+    q = torch.full((w, s, 64), a, dtype=dtype, device="cuda")
+    ref, mass, _, sv = _cross_reference(q, cache, None)
+    _check(kv8.cross_attn(q, cache), ref, mass, 0.0, sv, 2.0**-20)
+
+
+@pytest.mark.parametrize("dtype,a,b", _LARGE)
+@pytest.mark.parametrize("n,s,c", [(3, 1, 150), (200, 1, 70), (3, 20, 150), (2, 100, 100)])
+def test_self_scores_past_2_24(dtype, a, b, n, s, c):
+    """The same over cached slots, the new tokens below them, and at the new tokens alone (rows without slots)."""
+    h = 20 if n == 200 else 1
+    g = _gen(s + c)
+    qkv, cache, src = _self_case(g, n, s, h, c, 1, dtype)
+    low = torch.rand(c, generator=g, device="cuda") < 0.6
+    low[3] = low[40] = False
+    k = torch.where(low[:, None], _others(b), b).expand(n, h, c, 64).contiguous().to(dtype)
+    scale = torch.exp2(torch.ceil(torch.log2(k.float().abs().amax(-1) / 448)))
+    cache.k.copy_((k.float() / scale[..., None]).to(torch.float8_e4m3fn))
+    cache.k_scale.copy_(scale)
+    offset = torch.full((n,), c, device="cuda")
+    offset[0] = 0
+    q3 = qkv.unflatten(-1, (3, h, 64))
+    q3[:, :, 0] = a
+    q3[1:, :, 1] = _others(b)
+    q3[0, :, 1] = b
+    y = kv8.self_attn(qkv, cache, offset, src).unflatten(-1, (h, 64))
+    v = _values(cache, 1)[1]
+    q64 = qkv.double().unflatten(-1, (3, h, 64))
+    for r in (0, 1, n - 1):
+        m = int(offset[r])
+        for i in (0, s // 2, s - 1):
+            seen = v[r, :, :m][:, ~low[:m]] if m else q64[r, :i + 1, 2].transpose(0, 1)
+            _check(y[r, i], seen.mean(1), seen.abs().mean(1), 0.0, seen.abs().sum(1), 2.0**-16)

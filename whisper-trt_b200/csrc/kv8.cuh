@@ -126,6 +126,11 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // fp16 weights enter the products times 2^15 (the largest is then 2^15, and a unit's sums are divided by it again as
 // they are added): normal down to 2^-29 of the largest, and never off by more than 2^-40 of it.
 constexpr float kWeightExp = 15.f, kWeightInv = 1.f / 32768.f;
+// An exponent is score + (15 - maximum): one addition a weight. From maxima of 2^22 on the bracket rounds by more than 1/4,
+// and a weight could pass fp16's largest value: there the maximum is subtracted from the scores first, or the 15 left out.
+// (A row's own matter: the others' results do not change by it.)
+constexpr float kFarMax = 4194304.f;
+__device__ __forceinline__ float far_part(float b) { return fabsf(b) >= kFarMax ? b : 0.f; }
 
 // Queries enter the products as fp16 beside the fp16 form of the stored keys. fp16 queries do so as they are; a bf16
 // query is first divided by a power of two that brings its largest magnitude near 2^12, where fp16 holds all of its 8

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
     const int ahead = u + (STAGES - 1) * step;
     if (ahead < units) issue(ahead, stage == 0 ? STAGES - 1 : stage - 1);
     cp_commit_group();
-    const float k_now = ksc, v_now = vsc * kWeightInv;
+    const float k_now = ksc, v_now = vsc;
     if (u + step < units) {  // (the next unit's scales, while this one is worked on)
       ksc = ks[sbase + ((u + step) * kUnit) / kFrameBlock];
       vsc = vs[sbase + ((u + step) * kUnit) / kFrameBlock];
@@ -186,7 +186,10 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
           o[nt][i][3] *= al1;
         }
       }
-      const float up0 = kWeightExp - b0, up1 = kWeightExp - b1;
+      // (past kFarMax weights of at most 1, exact: what fp16 makes of them errs by 2^-25 of the largest)
+      const bool near0 = fabsf(b0) < kFarMax, near1 = fabsf(b1) < kFarMax;
+      const float up0 = (near0 ? kWeightExp : 0.f) - b0, up1 = (near1 ? kWeightExp : 0.f) - b1;
+      const float inv0 = near0 ? kWeightInv : 1.f, inv1 = near1 ? kWeightInv : 1.f;
       float tmp[4][4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) tmp[i][0] = tmp[i][1] = tmp[i][2] = tmp[i][3] = 0.f;
@@ -199,14 +202,15 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
         s1 += p1 + p3;
         unit_output(tmp, va[t], p0, p1, p2, p3);
       }
-      l[nt][0] = fmaf(s0, kWeightInv, l[nt][0]);
-      l[nt][1] = fmaf(s1, kWeightInv, l[nt][1]);
+      l[nt][0] = fmaf(s0, inv0, l[nt][0]);
+      l[nt][1] = fmaf(s1, inv1, l[nt][1]);
+      const float v0 = v_now * inv0, v1 = v_now * inv1;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        o[nt][i][0] = fmaf(tmp[i][0], v_now, o[nt][i][0]);
-        o[nt][i][1] = fmaf(tmp[i][1], v_now, o[nt][i][1]);
-        o[nt][i][2] = fmaf(tmp[i][2], v_now, o[nt][i][2]);
-        o[nt][i][3] = fmaf(tmp[i][3], v_now, o[nt][i][3]);
+        o[nt][i][0] = fmaf(tmp[i][0], v0, o[nt][i][0]);
+        o[nt][i][1] = fmaf(tmp[i][1], v1, o[nt][i][1]);
+        o[nt][i][2] = fmaf(tmp[i][2], v0, o[nt][i][2]);
+        o[nt][i][3] = fmaf(tmp[i][3], v1, o[nt][i][3]);
       }
     }
     __syncwarp();  // (every lane has read the stage before it is filled again)

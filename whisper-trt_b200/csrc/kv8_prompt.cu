@@ -125,7 +125,20 @@ __device__ __forceinline__ void prompt_block(float (&o)[8][4], float (&m)[2], fl
       o[i][3] *= a1;
     }
   }
-  const float up0 = up - (m[0] == kNegInf ? 0.f : m[0]), up1 = up - (m[1] == kNegInf ? 0.f : m[1]);
+  float b0 = m[0] == kNegInf ? 0.f : m[0], b1 = m[1] == kNegInf ? 0.f : m[1];
+  if (up != 0.f && __any_sync(0xffffffffu, fmaxf(fabsf(b0), fabsf(b1)) >= kFarMax)) {
+    const float f0 = far_part(b0), f1 = far_part(b1);
+#pragma unroll
+    for (int nt = 0; nt < 8; ++nt) {
+      sc[nt][0] -= f0;
+      sc[nt][1] -= f0;
+      sc[nt][2] -= f1;
+      sc[nt][3] -= f1;
+    }
+    b0 = fabsf(b0) >= kFarMax ? 0.f : b0;
+    b1 = fabsf(b1) >= kFarMax ? 0.f : b1;
+  }
+  const float up0 = up - b0, up1 = up - b1;
   // The keys that stand beside these queries: what a later token's value holds stays away from the earlier queries (a zero
   // weight alone would make NaN of it), so values that are not finite go around the product.
   const int beside = CACHED ? -1 : (qw0 - jb) >> 4;

@@ -184,7 +184,16 @@ __global__ void __launch_bounds__(kSWarps * 32, kSResident / kSWarps)
         o[i][3] *= al;
       }
     }
-    const float up = kWeightExp - (m == kNegInf ? 0.f : m);
+    float base = m == kNegInf ? 0.f : m;
+    if (fabsf(base) >= kFarMax) {  // (the same in all lanes)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        x[t][0] -= base;
+        x[t][1] -= base;
+      }
+      base = 0.f;
+    }
+    const float up = kWeightExp - base;
     float tmp[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tmp[i][0] = tmp[i][1] = tmp[i][2] = tmp[i][3] = 0.f;

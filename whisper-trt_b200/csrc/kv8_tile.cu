@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
     const size_t sbase = wh * ((a.T + kFrameBlock - 1) / kFrameBlock) + first;
     float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f}, vref = 1.f;
     float next_k = nb > 0 ? a.ks[sbase] : 0.f, next_v = nb > 0 ? a.vs[sbase] : 0.f;  // the next block's scales
-    bool ok = wait(q_full, 0);
+    bool ok = wait(q_full, 0), far = false;  // far: one of the warp's maxima is
     const float factor[2] = {ok ? q_fac[row0 + (lane >> 2)] : 0.f, ok ? q_fac[row0 + (lane >> 2) + 8] : 0.f};
     for (int i = 0; i < nb && ok; ++i) {
       const uint32_t at = tmem + rows + static_cast<uint32_t>(i % kTScores * kTK);
@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
           by[e] = al * (vref / vn);
         }
         vref = vn;
+        far = __any_sync(0xffffffffu, fmaxf(fabsf(m[0]), fabsf(m[1])) >= kFarMax);  // (-inf with them: it makes 0 of its base)
         if (i > 0) {  // the output so far, once block i - 1 is in it
           ok = wait(&pv_done[(i - 1) % kTScores], ((i - 1) / kTScores) & 1);
           if (!ok) break;
@@ -299,9 +300,20 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       // below 2^-81 of the largest.)
       int re = static_cast<int>(__float_as_uint(top) >> 23) - static_cast<int>(__float_as_uint(vref) >> 23);
       re = re < -90 ? -90 : re;
-      const float up[2] = {kUp - (m[0] == kNegInf ? 0.f : m[0]) + static_cast<float>(re),
-                           kUp - (m[1] == kNegInf ? 0.f : m[1]) + static_cast<float>(re)};
-      const Pair f2[2] = {pair_of(f[0], f[0]), pair_of(f[1], f[1])}, up2[2] = {pair_of(up[0], up[0]), pair_of(up[1], up[1])};
+      float base[2] = {m[0] == kNegInf ? 0.f : m[0], m[1] == kNegInf ? 0.f : m[1]}, by[2] = {f[0], f[1]};
+      if (far) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (fabsf(base[e]) >= kFarMax) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (((j >> 1) & 1) == e) x[j] = __fsub_rn(__fmul_rn(x[j], f[e]), base[e]);  // (rounded like the maxima)
+            base[e] = 0.f;
+            by[e] = 1.f;
+          }
+      }
+      const float up[2] = {kUp - base[0] + static_cast<float>(re), kUp - base[1] + static_cast<float>(re)};
+      const Pair f2[2] = {pair_of(by[0], by[0]), pair_of(by[1], by[1])}, up2[2] = {pair_of(up[0], up[0]), pair_of(up[1], up[1])};
       uint32_t hi[16], lo[16];
       Pair sum[2] = {0, 0};
 #pragma unroll
