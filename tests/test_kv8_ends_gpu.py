@@ -94,3 +94,34 @@ def test_self_scores_past_2_24(dtype, a, b, n, s, c):
         for i in (0, s // 2, s - 1):
             seen = v[r, :, :m][:, ~low[:m]] if m else q64[r, :i + 1, 2].transpose(0, 1)
             _check(y[r, i], seen.mean(1), seen.abs().mean(1), 0.0, seen.abs().sum(1), 2.0**-16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("s,t", [(5, 100), (20, 1500), (40, 100), (40, 1500)])
+def test_cross_scores_of_minus_infinity(dtype, s, t):
+    """A query all of whose scores are minus infinity has no softmax (NaN); the others, and windows without frames, have."""
+    g = _gen(s)
+    k, v = _randn(g, 3, 2, t, 64, dtype=dtype), _randn(g, 3, 2, t, 64, dtype=dtype)
+    k[..., 0] = k[..., 0].abs() + 1
+    q = _randn(g, 3, s, 128, dtype=dtype)
+    q[:, 1, 0] = -torch.inf
+    lengths = torch.tensor([t, 0, 70], device="cuda")
+    y = kv8.cross_attn(q, kv8.quantize_cross(k, v), lengths)
+    assert torch.isnan(y[[0, 2], 1, :64]).all() and (y[1] == 0).all()
+    y[:, 1, :64] = 0
+    assert torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("s", [1, 40])
+def test_self_scores_of_minus_infinity(dtype, s):
+    n, h, c = 3, 2, 90
+    qkv, cache, src = _self_case(_gen(s), n, s, h, c, 1, dtype)
+    cache.k.view(torch.uint8)[..., 0] &= 0x7F  # (keys at least 0 there: minus infinity, or NaN where they are 0)
+    q3 = qkv.unflatten(-1, (3, h, 64))
+    q3[..., 1, :, 0] = q3[..., 1, :, 0].abs() + 1
+    q3[1, s - 1, 0, 1, 0] = -torch.inf
+    y = kv8.self_attn(qkv, cache, torch.tensor([5, 60, 90], device="cuda"), src).unflatten(-1, (h, 64))
+    assert torch.isnan(y[1, s - 1, 1]).all()
+    y[1, s - 1, 1] = 0
+    assert torch.isfinite(y).all()

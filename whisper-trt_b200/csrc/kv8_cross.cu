@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
         num[7] = num[7] * wa + b.w * wb;
       }
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;  // (no frame: zeros)
+    const float inv = len == 0 ? 0.f : 1.f / den;  // (no frame: zeros; none but of score -inf: NaN)
 #pragma unroll
     for (int i = 0; i < 8; ++i) num[i] *= inv;
     *reinterpret_cast<uint4 *>(y + (static_cast<size_t>(w) * S + q0 + qq) * HD + static_cast<size_t>(h) * 64 + d8) =

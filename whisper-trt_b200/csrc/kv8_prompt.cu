@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kTThreads, 4) prompt8_kernel(const PromptArgs 
     l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
     l[1] += __shfl_xor_sync(0xffffffffu, l[1], x);
   }
-  const float r0 = l[0] == 0.f ? 0.f : 1.f / l[0], r1 = l[1] == 0.f ? 0.f : 1.f / l[1];  // (no frame: zeros)
+  const float r0 = 1.f / l[0], r1 = 1.f / l[1];  // (a query sees itself at least; nothing but scores of -inf: NaN)
   unsigned char *os = q_raw + warp * 16 * 128;
 #pragma unroll
   for (int dt = 0; dt < 8; ++dt) {

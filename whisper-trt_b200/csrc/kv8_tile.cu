@@ -347,24 +347,25 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
     if (ok && nb > 0) ok = wait(&pv_done[(nb - 1) % kTScores], ((nb - 1) / kTScores) & 1);
     if (ok) {
       tc_fence_after();
-      float f[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 2);
-        f[e] = l[e] == 0.f ? 0.f : vref / l[e];  // (nothing seen: zeros)
       }
       uint32_t o[32];
       if (nb > 0) {
         tmem_ld_rows64(tmem_o + rows, o);
         tmem_wait_ld();
+      } else {  // (no frame: zeros)
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = 0;
       }
       if constexpr (SHARED) {  // this CTA's share of the sums, over the tiles of keys that every MMA is done with
         float *to = reinterpret_cast<float *>(kv) + (row0 + (lane >> 2)) * kTRec + 2 * (lane & 3);
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           *reinterpret_cast<float2 *>(to + (j & 1) * 8 * kTRec + (j >> 1) * 8) =
-              nb > 0 ? make_float2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1])) : make_float2(0.f, 0.f);
+              make_float2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
         if ((lane & 3) == 0) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
@@ -375,13 +376,12 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
         }
       } else {  // by way of the query tile, which every MMA is done with, as whole pieces of rows
         unsigned char *to = qt + row0 * 128;
+        const float f[2] = {nb > 0 ? vref / l[0] : 0.f, nb > 0 ? vref / l[1] : 0.f};  // (nothing but scores of -inf: NaN)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int e = j & 1;
-          const float z0 = l[e] == 0.f ? 0.f : __uint_as_float(o[2 * j]) * f[e];
-          const float z1 = l[e] == 0.f ? 0.f : __uint_as_float(o[2 * j + 1]) * f[e];
           *reinterpret_cast<uint32_t *>(to + swz128((lane >> 2) + 8 * e, j >> 1) + 4 * (lane & 3)) =
-              Elem<T>::from_float2(z0, z1);
+              Elem<T>::from_float2(__uint_as_float(o[2 * j]) * f[e], __uint_as_float(o[2 * j + 1]) * f[e]);
         }
         __syncwarp();
         T *yr = static_cast<T *>(a.y) + (static_cast<size_t>(b) * a.S + q0 + row0) * HD + static_cast<size_t>(h) * 64;
@@ -521,9 +521,9 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
           num[6] = fmaf(wv, o[c][1].z, num[6]);
           num[7] = fmaf(wv, o[c][1].w, num[7]);
         }
-      const float f = den == 0.f ? 0.f : v / den;
+      const float f = all == 0 ? 0.f : v / den;  // (no frame: zeros; none but of score -inf: NaN)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) num[i] = den == 0.f ? 0.f : num[i] * f;
+      for (int i = 0; i < 8; ++i) num[i] *= f;
       *reinterpret_cast<uint4 *>(static_cast<T *>(a.y) + (static_cast<size_t>(b) * a.S + q0 + row) * HD +
                                  static_cast<size_t>(h) * 64 + d8) = pack8<T>(num);
     }
