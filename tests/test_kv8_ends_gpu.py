@@ -125,3 +125,23 @@ def test_self_scores_of_minus_infinity(dtype, s):
     assert torch.isnan(y[1, s - 1, 1]).all()
     y[1, s - 1, 1] = 0
     assert torch.isfinite(y).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("far", [30, 90])
+@pytest.mark.parametrize("w,s,t", [(20, 5, 300), (20, 40, 300), (1, 70, 700), (1, 130, 1500)])
+def test_cross_value_scales_far_apart(dtype, far, w, s, t):
+    """Blocks of values 2^`far` times the others', at frames that next to no weight falls on: what the weight does fall on keeps
+    its bits (errors are relative to a row's own sum of p |v|). Every third block, all but those, the first, the last."""
+    g = _gen(s + t + far)
+    q = _randn(g, w, s, 64, dtype=dtype)
+    q[..., 0] = 16
+    last = (t - 1) // 64
+    for big in ([b for b in range(last) if b % 3 == 1], [b for b in range(last) if b % 3 != 1], [0], [last]):
+        k = _randn(g, w, 1, t, 64, dtype=dtype)
+        k[..., 0] = 0
+        for b in big:
+            k[:, :, 64 * b:64 * b + 64, 0] = -0.4 * far - 16  # (weights of about 2^-(1.15 far + 46))
+        cache = kv8.quantize_cross(k, _randn(g, w, 1, t, 64, dtype=dtype))
+        cache.v_scale[:, :, big] *= 2.0**far
+        _check(kv8.cross_attn(q, cache), *_cross_reference(q, cache, None), 2.0**-20, least=0.0)

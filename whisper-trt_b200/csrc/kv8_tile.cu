@@ -21,9 +21,11 @@
 // two CTAs on an SM and three S in flight hide part of it. Fewer copies, one exponential for all, a stage more: 2 to 5%.
 //
 // Scales: a score is multiplied by the block's key scale and the query's power (query_exp), a weight by the block's
-// value scale over a reference, the largest one so far, by whose change the output is rescaled like a maximum's. Weights enter
-// as fp16, 2^kUp times themselves (at most 2^15), normal down to 2^-(14 + kUp) of the reference maximum and never off by
-// more than 2^-(25 + kUp) of it, in two parts, hi + lo, so that their rounding does not add to the output's. Waits are bounded as in the other tcgen05 kernels: a wait that runs out sets the error word and a stop flag.
+// value scale over the row's reference, which follows, like its maximum and as lazily, the largest product of a weight and a
+// value scale so far: a block of large values that no weight falls on costs the others no bits. Weights enter as fp16, 2^kUp
+// times themselves (at most 2^15), normal down to 2^-(14 + kUp) of the reference and never off by more than 2^-(25 + kUp) of
+// it, in two parts, hi + lo, so that their rounding does not add to the output's. Waits are bounded as in the other tcgen05
+// kernels: a wait that runs out sets the error word and a stop flag.
 #include <cooperative_groups.h>
 
 #include "kv8.cuh"
@@ -38,6 +40,7 @@ constexpr int kTQ = 128, kTK = 64;
 constexpr int kTSoftmax = 8, kTLoaders = 4, kTThreads = (kTSoftmax + kTLoaders + 1) * 32;  // warps; threads
 constexpr int kTQTile = kTQ * 128, kTKTile = kTK * 128;  // bytes: 128 or 64 rows of 64 16-bit values
 constexpr float kLag = 8.f, kUp = 7.f;                   // (kLag + kUp = 15: fp16's largest power of two)
+constexpr float kLow = -3e38f, kNoRef = -150.f;          // a row's maximum and value reference before any score: below all
 constexpr int kTErrTimeout = 1;
 constexpr int kTCluster = 4;
 constexpr int kTRec = 68;                                // floats of a row of a CTA's share (64, apart in the banks)
@@ -132,7 +135,7 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   __shared__ int lens[kTThreads], chosen;
   __shared__ float q_fac[kTQ];
-  __shared__ float state[3][SHARED ? kTQ : 1];  // this CTA's maxima, sums, value references
+  __shared__ float state[3][SHARED ? kTQ : 1];  // this CTA's rows' maxima, sums, value references
 
   if (warp == 0) {
     tmem_alloc(tmem_holder, kTTmem);
@@ -224,7 +227,8 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
     const int row0 = (warp & 3) * 32 + (warp >> 2) * 16;  // a warp reaches the 32 rows of its quarter: 16 of them its own
     const uint32_t rows = static_cast<uint32_t>(row0) << 16;
     const size_t sbase = wh * ((a.T + kFrameBlock - 1) / kFrameBlock) + first;
-    float m[2] = {kNegInf, kNegInf}, l[2] = {0.f, 0.f}, vref = 1.f;
+    // a row's maximum, sum and value reference (whole numbers in log2 units: moving them is exact)
+    float m[2] = {kLow, kLow}, l[2] = {0.f, 0.f}, ref[2] = {kNoRef, kNoRef};
     float next_k = nb > 0 ? a.ks[sbase] : 0.f, next_v = nb > 0 ? a.vs[sbase] : 0.f;  // the next block's scales
     bool ok = wait(q_full, 0), far = false;  // far: one of the warp's maxima is
     const float factor[2] = {ok ? q_fac[row0 + (lane >> 2)] : 0.f, ok ? q_fac[row0 + (lane >> 2) + 8] : 0.f};
@@ -232,7 +236,8 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       const uint32_t at = tmem + rows + static_cast<uint32_t>(i % kTScores * kTK);
       // (held above 0, where zero or tiny queries meet zero or tiny keys: frames that are not there are -inf before it)
       constexpr float kLeast = 1.17549435e-38f;
-      const float f[2] = {fmaxf(next_k * factor[0], kLeast), fmaxf(next_k * factor[1], kLeast)}, top = next_v;
+      float f[2] = {fmaxf(next_k * factor[0], kLeast), fmaxf(next_k * factor[1], kLeast)};
+      const float ve = static_cast<float>(static_cast<int>(__float_as_uint(next_v) >> 23) - 127);
       if (i + 1 < nb) {
         next_k = a.ks[sbase + i + 1];
         next_v = a.vs[sbase + i + 1];
@@ -246,7 +251,6 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       float x[32];
 #pragma unroll
       for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(raw[j]);
-      if (i == 0) vref = top;
       const int lim = len - 1 - i * kTK - 2 * (lane & 3);  // of this lane's columns, the last frame that is there
       if (len - i * kTK < kTK) {
 #pragma unroll
@@ -266,20 +270,19 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
         mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * f[e];  // (f > 0)
       }
-      const bool late = mx[0] > m[0] + kLag || mx[1] > m[1] + kLag || (m[0] == kNegInf && mx[0] > kNegInf) ||
-                        (m[1] == kNegInf && mx[1] > kNegInf);
-      if (__any_sync(0xffffffffu, late) || top > vref) {
-        const float vn = fmaxf(vref, top);
+      const bool late = mx[0] > m[0] + kLag || mx[1] > m[1] + kLag || mx[0] - m[0] + ve > ref[0] + kLag ||
+                        mx[1] - m[1] + ve > ref[1] + kLag;
+      if (__any_sync(0xffffffffu, late)) {
         float by[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float mn = fmaxf(m[e], mx[e]), al = ex2f(m[e] - (mn == kNegInf ? 0.f : mn));
-          l[e] *= al;
+          const float up = ceilf(mx[e]), mn = fmaxf(m[e], up), go = m[e] - mn, rn = fmaxf(ref[e] + go, up - mn + ve);
+          l[e] *= ex2f(go);
+          by[e] = ex2f(ref[e] + go - rn);
           m[e] = mn;
-          by[e] = al * (vref / vn);
+          ref[e] = rn;
         }
-        vref = vn;
-        far = __any_sync(0xffffffffu, fmaxf(fabsf(m[0]), fabsf(m[1])) >= kFarMax);  // (-inf with them: it makes 0 of its base)
+        far = __any_sync(0xffffffffu, fmaxf(fabsf(m[0]), fabsf(m[1])) >= kFarMax);
         if (i > 0) {  // the output so far, once block i - 1 is in it
           ok = wait(&pv_done[(i - 1) % kTScores], ((i - 1) / kTScores) & 1);
           if (!ok) break;
@@ -295,25 +298,23 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
           }
         }
       }
-      // Weights, over the scores that they come from. (The value scale's ratio to vref, a power of two, goes into the
-      // exponent, and out of the sum again. Below 2^-90 the weights themselves would leave fp32; what such values give is
-      // below 2^-81 of the largest.)
-      int re = static_cast<int>(__float_as_uint(top) >> 23) - static_cast<int>(__float_as_uint(vref) >> 23);
-      re = re < -90 ? -90 : re;
-      float base[2] = {m[0] == kNegInf ? 0.f : m[0], m[1] == kNegInf ? 0.f : m[1]}, by[2] = {f[0], f[1]};
+      // Weights, over the scores that they come from. (The value scale over the row's reference, a power of two, goes into
+      // the exponent, and out of the sum again. Below 2^-90 the weights themselves would leave fp32; what such values give
+      // is below 2^-81 of the largest.)
+      const float shift[2] = {fmaxf(ve - ref[0], -90.f), fmaxf(ve - ref[1], -90.f)};
+      float up[2] = {kUp - m[0] + shift[0], kUp - m[1] + shift[1]};
       if (far) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (fabsf(base[e]) >= kFarMax) {
+          if (fabsf(m[e]) >= kFarMax) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (((j >> 1) & 1) == e) x[j] = __fsub_rn(__fmul_rn(x[j], f[e]), base[e]);  // (rounded like the maxima)
-            base[e] = 0.f;
-            by[e] = 1.f;
+              if (((j >> 1) & 1) == e) x[j] = __fsub_rn(__fmul_rn(x[j], f[e]), m[e]);  // (rounded like the maxima)
+            f[e] = 1.f;
+            up[e] = kUp + shift[e];
           }
       }
-      const float up[2] = {kUp - base[0] + static_cast<float>(re), kUp - base[1] + static_cast<float>(re)};
-      const Pair f2[2] = {pair_of(by[0], by[0]), pair_of(by[1], by[1])}, up2[2] = {pair_of(up[0], up[0]), pair_of(up[1], up[1])};
+      const Pair f2[2] = {pair_of(f[0], f[0]), pair_of(f[1], f[1])}, up2[2] = {pair_of(up[0], up[0]), pair_of(up[1], up[1])};
       uint32_t hi[16], lo[16];
       Pair sum[2] = {0, 0};
 #pragma unroll
@@ -332,12 +333,11 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       }
       tmem_st_pairs(at, hi);
       tmem_st_pairs(at + 32, lo);
-      const float down = exp2_int(-re);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float s0, s1;
         halves(sum[e], s0, s1);
-        l[e] = fmaf(s0 + s1, down, l[e]);
+        l[e] = fmaf(s0 + s1, ex2f(-shift[e]), l[e]);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -371,17 +371,18 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
           for (int e = 0; e < 2; ++e) {
             state[0][row0 + (lane >> 2) + 8 * e] = m[e];
             state[1][row0 + (lane >> 2) + 8 * e] = l[e];
-            state[2][row0 + (lane >> 2) + 8 * e] = vref;
+            state[2][row0 + (lane >> 2) + 8 * e] = ref[e];
           }
         }
       } else {  // by way of the query tile, which every MMA is done with, as whole pieces of rows
         unsigned char *to = qt + row0 * 128;
-        const float f[2] = {nb > 0 ? vref / l[0] : 0.f, nb > 0 ? vref / l[1] : 0.f};  // (nothing but scores of -inf: NaN)
+        // (no frame: zeros; nothing but scores of -inf: NaN)
+        const float f[2] = {nb > 0 ? 1.f / l[0] : 0.f, nb > 0 ? 1.f / l[1] : 0.f}, r[2] = {ex2f(ref[0]), ex2f(ref[1])};
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int e = j & 1;
           *reinterpret_cast<uint32_t *>(to + swz128((lane >> 2) + 8 * e, j >> 1) + 4 * (lane & 3)) =
-              Elem<T>::from_float2(__uint_as_float(o[2 * j]) * f[e], __uint_as_float(o[2 * j + 1]) * f[e]);
+              Elem<T>::from_float2(__uint_as_float(o[2 * j]) * f[e] * r[e], __uint_as_float(o[2 * j + 1]) * f[e] * r[e]);
         }
         __syncwarp();
         T *yr = static_cast<T *>(a.y) + (static_cast<size_t>(b) * a.S + q0 + row0) * HD + static_cast<size_t>(h) * 64;
@@ -487,7 +488,7 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       const int row = t >> 3, d8 = (t & 7) * 8;
       if (q0 + row >= a.S) continue;
       float4 o[kTCluster][2];
-      float m[kTCluster], l[kTCluster], r[kTCluster], top = kNegInf, v = 0.f, den = 0.f;
+      float m[kTCluster], l[kTCluster], r[kTCluster], top = kLow, v = kNoRef, den = 0.f;
 #pragma unroll
       for (int c = 0; c < kTCluster; ++c) {  // (all loads together)
         const int from = c < cl ? c : rank;
@@ -503,14 +504,14 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
       float num[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < kTCluster; ++c)
-        if (l[c] != 0.f) {  // (it has seen a frame)
-          top = fmaxf(top, m[c]);
-          v = fmaxf(v, r[c]);
-        }
+        if (l[c] != 0.f) top = fmaxf(top, m[c]);  // (it has seen a frame)
+#pragma unroll
+      for (int c = 0; c < kTCluster; ++c)
+        if (l[c] != 0.f) v = fmaxf(v, m[c] - top + r[c]);
 #pragma unroll
       for (int c = 0; c < kTCluster; ++c)
         if (l[c] != 0.f) {
-          const float w = ex2f(m[c] - (top == kNegInf ? 0.f : top)), wv = w * (r[c] / v);
+          const float w = ex2f(m[c] - top), wv = ex2f(m[c] - top + r[c] - v);
           den = fmaf(w, l[c], den);
           num[0] = fmaf(wv, o[c][0].x, num[0]);
           num[1] = fmaf(wv, o[c][0].y, num[1]);
@@ -521,9 +522,9 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
           num[6] = fmaf(wv, o[c][1].z, num[6]);
           num[7] = fmaf(wv, o[c][1].w, num[7]);
         }
-      const float f = all == 0 ? 0.f : v / den;  // (no frame: zeros; none but of score -inf: NaN)
+      const float f = all == 0 ? 0.f : 1.f / den, by = ex2f(v);  // (no frame: zeros; none but of score -inf: NaN)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) num[i] *= f;
+      for (int i = 0; i < 8; ++i) num[i] = num[i] * f * by;
       *reinterpret_cast<uint4 *>(static_cast<T *>(a.y) + (static_cast<size_t>(b) * a.S + q0 + row) * HD +
                                  static_cast<size_t>(h) * 64 + d8) = pack8<T>(num);
     }
