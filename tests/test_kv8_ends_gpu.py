@@ -145,3 +145,28 @@ def test_cross_value_scales_far_apart(dtype, far, w, s, t):
         cache = kv8.quantize_cross(k, _randn(g, w, 1, t, 64, dtype=dtype))
         cache.v_scale[:, :, big] *= 2.0**far
         _check(kv8.cross_attn(q, cache), *_cross_reference(q, cache, None), 2.0**-20, least=0.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("far", [30, 90])
+@pytest.mark.parametrize("n,s", [(3, 1), (200, 1), (3, 20)])
+def test_self_value_scales_far_apart(dtype, far, n, s):
+    """The same of slots next to one another."""
+    h, c = (20, 70) if n == 200 else (1, 150)
+    qkv, cache, src = _self_case(_gen(s + far), n, s, h, c, 1, dtype)
+    big = torch.arange(2, c, 5, device="cuda")
+    cache.v_scale[:, :, big] *= 2.0**far
+    cache.k_scale[:, :, big] = 2.0**-3
+    cache.k.view(torch.uint8)[..., 0] = 0
+    cache.k.view(torch.uint8)[:, :, big, 0] = 0xFE  # (-448: -56 with the scale)
+    q3 = qkv.unflatten(-1, (3, h, 64))
+    q3[:, :, 0, :, 0] = 0.0625 * far + 8  # (weights of 2^-100 and 2^-137)
+    q3[:, :, 1, :, 0] = 0
+    y = kv8.self_attn(qkv, cache, torch.full((n,), c, device="cuda"), src).unflatten(-1, (h, 64))
+    k, v = _values(cache, 1)
+    q64 = qkv.double().unflatten(-1, (3, h, 64))
+    for r in (0, n - 1):
+        for j in (0, h - 1):
+            for i in (0, s - 1):
+                kr, vr = (torch.cat((x[r, j], q64[r, :i + 1, 1 + e, j])) for e, x in enumerate((k, v)))
+                _check(y[r, i:i + 1, j], *_attend(q64[r, i:i + 1, 0, j], kr[None], vr[None]), 2.0**-16, least=0.0)

@@ -8,8 +8,9 @@
 // units go round the warps, through a ring of asynchronous copies per warp, the slot-table entries of a unit loaded one
 // unit earlier. The unit runs on mma.sync although there is a single query (all 8 columns hold it): converting 16 keys for the tensor cores and reading one column back takes 9 instructions a key, where
 // dot products and weighted sums on FMAs took 28 and bound the kernel (160 rows x 20 heads x 335 slots: 41 us).
-// Scales differ from slot to slot: a score is multiplied by its key's, a weight by its value's over the unit's largest
-// (at most 1), whose factor the unit's output takes as it is added. The new token is attended in fp32. The warps' states
+// Scales differ from slot to slot: a score is multiplied by its key's, a weight by its value's, and the unit's products by
+// the power of two that brings the largest of them near fp16's largest value, whose inverse the unit's output takes as it is
+// added: a slot of large values that no weight falls on costs the others no bits. The new token is attended in fp32. The warps' states
 // meet in shared memory, a cluster's through distributed shared memory.
 #include <cooperative_groups.h>
 
@@ -167,11 +168,6 @@ __global__ void __launch_bounds__(kSWarps * 32, kSResident / kSWarps)
     float mx = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
 #pragma unroll
     for (int s = 4; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-    // (scales are positive: their bits are in their order; past the end they are 0)
-    const float big = __uint_as_float(__reduce_max_sync(
-        0xffffffffu, max(max(__float_as_uint(w[0][0]), __float_as_uint(w[0][1])),
-                         max(__float_as_uint(w[1][0]), __float_as_uint(w[1][1])))));
-    const float inv = __uint_as_float(0x7f000000u - __float_as_uint(big));  // 1 / a power of two
     if (mx > m) {  // (the same in all lanes; rarer and rarer)
       const float al = ex2f(m - mx);
       m = mx;
@@ -184,30 +180,30 @@ __global__ void __launch_bounds__(kSWarps * 32, kSResident / kSWarps)
         o[i][3] *= al;
       }
     }
-    float base = m == kNegInf ? 0.f : m;
-    if (fabsf(base) >= kFarMax) {  // (the same in all lanes)
+    const float base = m == kNegInf ? 0.f : m;
+    float sum = 0.f;
+    uint32_t top = 0;  // (not negative: their bits are in their order)
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        x[t][0] -= base;
-        x[t][1] -= base;
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float p = ex2f(x[t][e] - base);
+        sum += p;
+        w[t][e] *= p;
+        top = max(top, __float_as_uint(w[t][e]));
       }
-      base = 0.f;
-    }
-    const float up = kWeightExp - base;
+    l += sum;
+    // the power of two that brings the largest into 2^14 .. 2^15 (of 2^-112 at least), and its inverse
+    const uint32_t big = max(__reduce_max_sync(0xffffffffu, top) >> 23 & 0xffu, 15u);
+    const float inv = __uint_as_float((127u + 14u + 127u - big) << 23), by = __uint_as_float((big - 14u) << 23);
     float tmp[4][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) tmp[i][0] = tmp[i][1] = tmp[i][2] = tmp[i][3] = 0.f;
-    float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      float p0 = ex2f(x[t][0] + up), p1 = ex2f(x[t][1] + up);
-      sum += p0 + p1;
-      p0 *= w[t][0] * inv;
-      p1 *= w[t][1] * inv;
+      const float p0 = w[t][0] * inv, p1 = w[t][1] * inv;
       unit_output(tmp, va[t], p0, p0, p1, p1);
     }
-    l = fmaf(sum, kWeightInv, l);
-    const float by = big * kWeightInv;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
