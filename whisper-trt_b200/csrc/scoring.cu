@@ -101,7 +101,8 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const LpA
   extern __shared__ uint32_t bits[];  // the suppressed tokens of this CTA's pieces
   __shared__ LpShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int rank = blockIdx.x % a.cl, cid = blockIdx.x / a.cl, ncl = gridDim.x / a.cl;
+  const int rank = blockIdx.x % a.cl;
+  const uint32_t cid = blockIdx.x / a.cl, ncl = gridDim.x / a.cl;
 
   pdl_wait();
   pdl_launch_dependents();
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(kLpThreads, kLpCtas) logprobs_kernel(const LpA
   }
   auto suppressed = [&](int v) { return (bits[(v - bit0) >> 5] >> ((v - bit0) & 31)) & 1u; };
 
-  for (int row = cid; row < a.rows; row += ncl) {
+  for (uint32_t row = cid; row < static_cast<uint32_t>(a.rows); row += ncl) {  // (rows < 2^31, ncl <= 2^30: no wrap)
     const T *x = static_cast<const T *>(a.logits) + row * a.stride;
     const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));  // piece 0 starts here
     // piece p: tokens p * n - shift .. + n - 1; `count` pieces from p0 on, the first and last may be cut short
@@ -285,7 +286,7 @@ template <typename T, bool MASKED>
 int launch_logprobs(LpArgs a, int sms, void *stream) {
   // CTAs per row: as many as keep about 2 CTAs on every SM, and at least a round of pieces for each
   a.cl = 1;
-  while (a.cl < kLpMaxCluster && a.rows * a.cl * 2 <= 2 * sms && a.vocab >= a.cl * 2 * kLpThreads * Piece<T>::n) a.cl *= 2;
+  while (a.cl < kLpMaxCluster && a.rows <= sms / a.cl && a.vocab >= a.cl * 2 * kLpThreads * Piece<T>::n) a.cl *= 2;
   // with suppressed tokens a CTA's rows share the bits it makes of them; without, a CTA is a row
   constexpr int kMaxGrid = 1 << 30;
   int ncl = a.rows < kMaxGrid ? a.rows : kMaxGrid;
