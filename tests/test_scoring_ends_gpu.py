@@ -28,3 +28,21 @@ def test_logprobs_rows_past_2_30(suppress):
         return
     assert (got[:-2] == got[0]).all() and abs(got[0].item() + math.log(2)) < 1e-6
     assert abs(got[-2].item() + math.log1p(math.exp(-2))) < 1e-6 and got[-1] == got[0]
+
+
+@pytest.mark.parametrize("n", [4100, 6000])
+def test_score_rows_in_passes_over_one_scratch(n):
+    """Rows and alternatives enough to pass the scratch's bound; every row right, and the same bits every time, captured too."""
+    x, w, tokens, sup = _states(n, 51866, 64, torch.float16, n, True)
+    tokens[5] = -100
+    got = scoring.score_tokens(x, w, tokens, 16, sup)
+    for a in range(0, n, 1500):
+        part = slice(a, a + 1500)
+        _check(scoring.TokenScores(*(y[part] for y in got)), x[part].double() @ w.double().t(), tokens[part], 16, sup)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = scoring.score_tokens(x, w, tokens, 16, sup)
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(u, z) for u, z in zip(again, got))
+    assert attn_plugin.workspace_errors() == 0

@@ -533,12 +533,64 @@ size_t sl_bytes(const SlPlan &p, int rows) {
   return sl_token_bytes(rows) + static_cast<size_t>((rows + 31) / 32 * 32) * p.parts * p.rec * sizeof(float);
 }
 
+// Rows a pass of the two kernels takes: all of them, or as many equal shares (of whole 256-row blocks) as keep the scratch
+// within kSlScratch, which a pass of 7136 rows with 5 alternatives fits; the passes use it in turn.
+constexpr size_t kSlScratch = 320u << 20;
+int sl_pass_rows(int rows, int vocab, int d, int top, int sms, SlPlan *plan) {
+  int take = rows;
+  *plan = sl_plan(take, vocab, d, top, sms);
+  for (long long n = 2; sl_bytes(*plan, take) > kSlScratch && take > 2 * kSlRows; ++n) {
+    const long long least = static_cast<long long>((sl_bytes(*plan, take) + kSlScratch - 1) / kSlScratch) * rows / take;
+    n = n > least ? n : least;
+    take = static_cast<int>((rows + n - 1) / n + 2 * kSlRows - 1) / (2 * kSlRows) * (2 * kSlRows);
+    *plan = sl_plan(take, vocab, d, top, sms);
+  }
+  return take;
+}
+
 template <bool BF16, int KK>
 int launch_score(const CUtensorMap &wm, const CUtensorMap &xm, const SlArgs &a, void *stream) {
   const int st = opt_in_smem<score_kernel<BF16, KK>>(kSlSmem, "score_tokens");
   if (st != WT_OK) return st;
   return launch_clustered("score_tokens", score_kernel<BF16, KK>, dim3(2 * a.p.pairs), dim3(kSlThreads), kSlSmem, stream,
                           2, wm, xm, a);
+}
+
+// The same cut of the vocabulary for fewer rows (a call's last pass: the others' scratch holds it).
+SlPlan sl_with_rows(SlPlan p, int rows) {
+  p.mblk = (rows + 2 * kSlRows - 1) / (2 * kSlRows);
+  p.items = p.slices * p.mblk;
+  p.pairs = p.items < p.pairs ? p.items : p.pairs;
+  return p;
+}
+
+// One pass: x [a.N, d] (16-bit values of either type).
+int score_rows(int dtype, const uint16_t *x, const void *w, int d, const SlArgs &a, const ScoreOut &out, void *stream) {
+  CUtensorMap wm, xm;
+  int st = encode_tile_map(&wm, w, static_cast<unsigned long long>(a.V), static_cast<unsigned long long>(d), a.p.nmma / 2,
+                           dtype);
+  if (st != WT_OK) return st;
+  st = encode_tile_map(&xm, x, static_cast<unsigned long long>(a.N), static_cast<unsigned long long>(d), kSlRows, dtype);
+  if (st != WT_OK) return st;
+  const bool bf = dtype == WT_BF16;
+#define WT_SCORE_CASE(kk) st = bf ? launch_score<true, kk>(wm, xm, a, stream) : launch_score<false, kk>(wm, xm, a, stream)
+  if (a.top == 0)
+    WT_SCORE_CASE(0);
+  else if (a.top == 1)
+    WT_SCORE_CASE(1);
+  else if (a.top <= 4)
+    WT_SCORE_CASE(4);
+  else if (a.top <= 8)
+    WT_SCORE_CASE(8);
+  else
+    WT_SCORE_CASE(16);
+#undef WT_SCORE_CASE
+  if (st != WT_OK) return st;
+  // (with 5 alternatives of 51866 tokens, us of the whole call by a warp / a CTA a row: 160 rows x 136 records 48.9 / 44.5,
+  // 512 x 74 82.2 / 82.1, 1024 x 36 124 / 134, 7136 x 58 829 / 864)
+  if (a.p.parts <= 64)
+    return launch("score_tokens", score_merge_kernel, dim3((a.N + 3) / 4), dim3(128), 0, stream, a, out);
+  return launch("score_tokens", score_merge_wide_kernel, dim3(a.N), dim3(256), 0, stream, a, out);
 }
 
 }  // namespace
@@ -548,7 +600,9 @@ extern "C" size_t wt_score_tokens_workspace(int rows, int vocab, int d_model, in
   using namespace wt;
   if (rows <= 0 || vocab <= 0 || d_model <= 0 || top < 0 || top > kMaxTop) return 0;
   const int sms = device_sm_count();
-  return sl_bytes(sl_plan(rows, vocab, d_model, top, sms > 0 ? sms : 148), rows);
+  SlPlan p;
+  const int take = sl_pass_rows(rows, vocab, d_model, top, sms > 0 ? sms : 148, &p);
+  return sl_bytes(p, take);
 }
 
 extern "C" int wt_score_tokens(int dtype, const void *x, const void *w, const int64_t *tokens, const uint8_t *suppress,
@@ -570,38 +624,23 @@ extern "C" int wt_score_tokens(int dtype, const void *x, const void *w, const in
   WT_REQUIRE(dtype == WT_F16 || dtype == WT_BF16, WT_ERR_DTYPE, "score_tokens: unknown dtype %d", dtype);
   const int sms = device_sm_count();
   if (sms <= 0) return WT_ERR_CUDA;
-  const SlPlan p = sl_plan(rows, vocab, d_model, top, sms);
-  WT_REQUIRE(workspace && workspace_bytes >= sl_bytes(p, rows), WT_ERR_WORKSPACE,
-             "score_tokens: needs a workspace of %zu bytes (given %zu)", sl_bytes(p, rows),
+  SlPlan p;
+  const int take = sl_pass_rows(rows, vocab, d_model, top, sms, &p);
+  WT_REQUIRE(workspace && workspace_bytes >= sl_bytes(p, take), WT_ERR_WORKSPACE,
+             "score_tokens: needs a workspace of %zu bytes (given %zu)", sl_bytes(p, take),
              workspace ? workspace_bytes : 0);
-  CUtensorMap wm, xm;
-  int st = encode_tile_map(&wm, w, static_cast<unsigned long long>(vocab), static_cast<unsigned long long>(d_model),
-                           p.nmma / 2, dtype);
-  if (st != WT_OK) return st;
-  st = encode_tile_map(&xm, x, static_cast<unsigned long long>(rows), static_cast<unsigned long long>(d_model), kSlRows,
-                       dtype);
-  if (st != WT_OK) return st;
   unsigned char *ws = static_cast<unsigned char *>(workspace);
-  const SlArgs a{tokens, suppress, reinterpret_cast<float *>(ws + sl_token_bytes(rows)), reinterpret_cast<float *>(ws),
-                 rows,   vocab,    top, p, err, wait_limit(), test_withhold_stage()};
-  const bool bf = dtype == WT_BF16;
-#define WT_SCORE_CASE(kk) st = bf ? launch_score<true, kk>(wm, xm, a, stream) : launch_score<false, kk>(wm, xm, a, stream)
-  if (top == 0)
-    WT_SCORE_CASE(0);
-  else if (top == 1)
-    WT_SCORE_CASE(1);
-  else if (top <= 4)
-    WT_SCORE_CASE(4);
-  else if (top <= 8)
-    WT_SCORE_CASE(8);
-  else
-    WT_SCORE_CASE(16);
-#undef WT_SCORE_CASE
-  if (st != WT_OK) return st;
-  const ScoreOut out{logprob, entropy, top_logprob, top_token};
-  // (with 5 alternatives of 51866 tokens, us of the whole call by a warp / a CTA a row: 160 rows x 136 records 48.9 / 44.5,
-  // 512 x 74 82.2 / 82.1, 1024 x 36 124 / 134, 7136 x 58 829 / 864)
-  if (p.parts <= 64)
-    return launch("score_tokens", score_merge_kernel, dim3((rows + 3) / 4), dim3(128), 0, stream, a, out);
-  return launch("score_tokens", score_merge_wide_kernel, dim3(rows), dim3(256), 0, stream, a, out);
+  int st = WT_OK;
+  for (int row = 0; row < rows && st == WT_OK; row += take) {
+    const int n = rows - row < take ? rows - row : take;
+    const SlArgs a{tokens + row, suppress, reinterpret_cast<float *>(ws + sl_token_bytes(take)),
+                   reinterpret_cast<float *>(ws), n, vocab, top, n == take ? p : sl_with_rows(p, n), err, wait_limit(),
+                   test_withhold_stage()};
+    const size_t at = static_cast<size_t>(row);
+    st = score_rows(dtype, static_cast<const uint16_t *>(x) + at * d_model, w, d_model, a,
+                    ScoreOut{logprob + at, entropy + at, top ? top_logprob + at * top : nullptr,
+                             top ? top_token + at * top : nullptr},
+                    stream);
+  }
+  return st;
 }
