@@ -170,3 +170,14 @@ def test_self_value_scales_far_apart(dtype, far, n, s):
             for i in (0, s - 1):
                 kr, vr = (torch.cat((x[r, j], q64[r, :i + 1, 1 + e, j])) for e, x in enumerate((k, v)))
                 _check(y[r, i:i + 1, j], *_attend(q64[r, i:i + 1, 0, j], kr[None], vr[None]), 2.0**-16, least=0.0)
+
+
+@pytest.mark.parametrize("s", [2097121, 4000000])
+def test_cross_queries_past_2_21(s):
+    """One window and head, more queries than a grid has rows of 32 for."""
+    g = _gen(s)
+    cache = kv8.quantize_cross(_randn(g, 1, 1, 70, 64, dtype=torch.float16), _randn(g, 1, 1, 70, 64, dtype=torch.float16))
+    q = torch.randn(1, s, 64, generator=g, device="cuda", dtype=torch.float16)
+    y = kv8.cross_attn(q, cache)
+    pick = torch.tensor([0, 1, s // 2, s - 129, s - 2, s - 1], device="cuda")
+    _check(y[:, pick], *_cross_reference(q[:, pick], cache, None), 2.0**-20)

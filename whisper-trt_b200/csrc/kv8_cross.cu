@@ -38,7 +38,6 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
   const int g = lane >> 2, c = lane & 3;
   const int wh = blockIdx.x / cl, rank = blockIdx.x - wh * cl;
   const int w = wh / H, h = wh - w * H;
-  const int q0 = blockIdx.y * NT * 8;
   unsigned char *ring = smem + warp * kRing;
 
   pdl_wait();
@@ -86,7 +85,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
   float qs[NT][2];  // the factors of the scores of queries 2c and 2c + 1
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int qi = q0 + nt * 8 + g;
+    const int qi = nt * 8 + g;
     uint4 a = make_uint4(0, 0, 0, 0), b = a;
     if (qi < S) {
       a = ldg16(qw + static_cast<size_t>(qi) * HD);
@@ -247,8 +246,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
   else
     __syncthreads();
   // all states -> the output: 8 threads a query, 8 head dims each; a cluster's CTAs share the (query, dims) items
-  const int nq = min(S - q0, NT * 8);
-  for (int t = rank * WARPS * 32 + threadIdx.x; t < nq * 8; t += cl * WARPS * 32) {
+  for (int t = rank * WARPS * 32 + threadIdx.x; t < S * 8; t += cl * WARPS * 32) {
     const int qq = t >> 3, d8 = (t & 7) * 8;
     float top = kNegInf, den = 0.f, num[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int cr = 0; cr < cl; ++cr) {
@@ -275,7 +273,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
     const float inv = len == 0 ? 0.f : 1.f / den;  // (no frame: zeros; none but of score -inf: NaN)
 #pragma unroll
     for (int i = 0; i < 8; ++i) num[i] *= inv;
-    *reinterpret_cast<uint4 *>(y + (static_cast<size_t>(w) * S + q0 + qq) * HD + static_cast<size_t>(h) * 64 + d8) =
+    *reinterpret_cast<uint4 *>(y + (static_cast<size_t>(w) * S + qq) * HD + static_cast<size_t>(h) * 64 + d8) =
         pack8<T>(num);
   }
   if (cl > 1) cluster.sync();  // (no CTA leaves while another reads its records)
@@ -289,7 +287,7 @@ int launch_cross8(const void *q, const void *k8, const void *v8, const float *ks
   const int st = opt_in_smem<cross8_kernel<T, NT, WARPS, STAGES>>(smem, "kv8_cross_attn");
   if (st != WT_OK) return st;
   const float scale = static_cast<float>(0.125 * 1.4426950408889634);
-  const dim3 grid(W * H * cl, (S + NT * 8 - 1) / (NT * 8)), block(WARPS * 32);
+  const dim3 grid(W * H * cl), block(WARPS * 32);
   const int nblk = (Tn + kFrameBlock - 1) / kFrameBlock;
   if (cl > 1)
     return launch_clustered("kv8_cross_attn", kernel, grid, block, smem, stream, cl, static_cast<const T *>(q),
@@ -303,8 +301,8 @@ int launch_cross8(const void *q, const void *k8, const void *v8, const float *ks
 template <typename T>
 int cross8(const void *q, const void *k8, const void *v8, const float *ks, const float *vs, const int64_t *lengths,
            void *y, int W, int S, int H, int Tn, int sms, void *stream) {
-  const int nt = S <= 32 ? (S + 7) / 8 : 4;
-  const long long units = static_cast<long long>(W) * H * ((S + nt * 8 - 1) / (nt * 8));
+  const int nt = (S + 7) / 8;  // tiles of 8 queries: 1 to 4
+  const long long units = static_cast<long long>(W) * H;
   // CTAs per (window, head): 2 or 4 where the SMs then still hold them all, and a warp has a few units left. Measured at 20
   // heads x 1500 frames x 5 queries, fp16 (us per launch), by 1 / 2 / 4 / 8 CTAs: 1 window - / 7.3 / 6.3 / 8.0; 8
   // windows - / 11.3 / 11.8 / -; 32 windows 24.8 / 33 (of 3 warps' rings) / - / -.
@@ -342,7 +340,8 @@ extern "C" int wt_kv8_cross_attn(int dtype, const void *q, const void *k8, const
   WT_REQUIRE(head_dim == 64, WT_ERR_UNSUPPORTED, "kv8_cross_attn: head_dim %d (supported: 64)", head_dim);
   WT_REQUIRE(static_cast<long long>(windows) * heads < (1LL << 27), WT_ERR_ARG,
              "kv8_cross_attn: grid too large (windows %d x heads %d)", windows, heads);
-  WT_REQUIRE(queries <= 65535 * 32, WT_ERR_ARG, "kv8_cross_attn: too many queries (%d)", queries);
+  WT_REQUIRE(queries < (1 << 30) && static_cast<long long>(windows) * heads * kv8_cross_tiles(queries) < (1LL << 30),
+             WT_ERR_ARG, "kv8_cross_attn: too many queries (%d windows x %d heads x %d)", windows, heads, queries);
   const int sms = device_sm_count();
   if (sms <= 0) return WT_ERR_CUDA;
   // Up to 32 queries share one read of the keys here, and the tile kernel's 128 rows would be mostly empty. Measured (us, here

@@ -36,7 +36,7 @@
 namespace wt {
 namespace {
 
-constexpr int kTQ = 128, kTK = 64;
+constexpr int kTQ = kTileQueries, kTK = 64;
 constexpr int kTSoftmax = 8, kTLoaders = 4, kTThreads = (kTSoftmax + kTLoaders + 1) * 32;  // warps; threads
 constexpr int kTQTile = kTQ * 128, kTKTile = kTK * 128;  // bytes: 128 or 64 rows of 64 16-bit values
 constexpr float kLag = 8.f, kUp = 7.f;                   // (kLag + kUp = 15: fp16's largest power of two)
@@ -537,9 +537,8 @@ __global__ void __launch_bounds__(kTThreads, 2) tile8_kernel(const TileArgs a) {
 
 template <typename T>
 int launch_tile(TileArgs a, int sms, void *stream) {
-  a.tiles = (a.S + kTQ - 1) / kTQ;
-  const long long units = static_cast<long long>(a.W) * a.H * a.tiles;
-  WT_REQUIRE(units < (1LL << 30), WT_ERR_ARG, "kv8_cross_attn: too many queries (%d windows x %d)", a.W, a.S);
+  a.tiles = static_cast<int>(kv8_cross_tiles(a.S));
+  const long long units = static_cast<long long>(a.W) * a.H * a.tiles;  // (fewer than 2^30)
   // CTAs per tile of queries, a cluster that shares its frames: as many as two on each SM hold, of 3 blocks at least. Measured
   // (us, 20 heads x 1500 frames, fp16, with / without): 1 window x 64 queries 14.5 / 25.8, x 223 20.5 / 26.3, x 448 26.7 /
   // 33; 2 windows x 128 21.0 / 26.2; 4 windows x 64, one more per SM than without, 25.9 / 26.5.
