@@ -130,6 +130,7 @@ constexpr float kWeightExp = 15.f, kWeightInv = 1.f / 32768.f;
 // and a weight could pass fp16's largest value: there the maximum is subtracted from the scores first, or the 15 left out.
 // (A row's own matter: the others' results do not change by it.)
 constexpr float kFarMax = 4194304.f;
+constexpr float kLowest = -3.402823466e38f;  // a maximum before any score: no score but -inf is below it
 __device__ __forceinline__ float far_part(float b) { return fabsf(b) >= kFarMax ? b : 0.f; }
 
 // Queries enter the products as fp16 beside the fp16 form of the stored keys. fp16 queries do so as they are; a bf16

@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
   float m[NT][2], l[NT][2], o[NT][4][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    m[nt][0] = m[nt][1] = kNegInf;
+    m[nt][0] = m[nt][1] = kLowest;
     l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.f;
@@ -170,9 +170,8 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
         mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, x));
       }
       const float mn0 = fmaxf(m[nt][0], mx0), mn1 = fmaxf(m[nt][1], mx1);
-      const float b0 = mn0 == kNegInf ? 0.f : mn0, b1 = mn1 == kNegInf ? 0.f : mn1;
       if (__any_sync(0xffffffffu, mn0 != m[nt][0] || mn1 != m[nt][1])) {  // (rarer and rarer)
-        const float al0 = ex2f(m[nt][0] - b0), al1 = ex2f(m[nt][1] - b1);
+        const float al0 = ex2f(m[nt][0] - mn0), al1 = ex2f(m[nt][1] - mn1);
         m[nt][0] = mn0;
         m[nt][1] = mn1;
         l[nt][0] *= al0;
@@ -186,8 +185,8 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
         }
       }
       // (past kFarMax weights of at most 1, exact: what fp16 makes of them errs by 2^-25 of the largest)
-      const bool near0 = fabsf(b0) < kFarMax, near1 = fabsf(b1) < kFarMax;
-      const float up0 = (near0 ? kWeightExp : 0.f) - b0, up1 = (near1 ? kWeightExp : 0.f) - b1;
+      const bool near0 = fabsf(mn0) < kFarMax, near1 = fabsf(mn1) < kFarMax;
+      const float up0 = (near0 ? kWeightExp : 0.f) - mn0, up1 = (near1 ? kWeightExp : 0.f) - mn1;
       const float inv0 = near0 ? kWeightInv : 1.f, inv1 = near1 ? kWeightInv : 1.f;
       float tmp[4][4];
 #pragma unroll
@@ -248,7 +247,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
   // all states -> the output: 8 threads a query, 8 head dims each; a cluster's CTAs share the (query, dims) items
   for (int t = rank * WARPS * 32 + threadIdx.x; t < S * 8; t += cl * WARPS * 32) {
     const int qq = t >> 3, d8 = (t & 7) * 8;
-    float top = kNegInf, den = 0.f, num[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    float top = kLowest, den = 0.f, num[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     for (int cr = 0; cr < cl; ++cr) {
       const unsigned char *peer = cl > 1 ? cluster.map_shared_rank(smem, cr) : smem;
 #pragma unroll
@@ -256,8 +255,7 @@ __global__ void __launch_bounds__(WARPS * 32, few_ctas(NT))
         const float *r = reinterpret_cast<const float *>(peer + wi * kRing) + qq * kRec;
         const float mr = r[64], lr = r[65];
         const float4 a = *reinterpret_cast<const float4 *>(r + d8), b = *reinterpret_cast<const float4 *>(r + d8 + 4);
-        const float mn = fmaxf(top, mr), mu = mn == kNegInf ? 0.f : mn;
-        const float wa = ex2f(top - mu), wb = ex2f(mr - mu);
+        const float mn = fmaxf(top, mr), wa = ex2f(top - mn), wb = ex2f(mr - mn);
         top = mn;
         den = den * wa + lr * wb;
         num[0] = num[0] * wa + a.x * wb;
