@@ -46,3 +46,18 @@ def test_score_rows_in_passes_over_one_scratch(n):
         graph.replay()
         assert all(torch.equal(u, z) for u, z in zip(again, got))
     assert attn_plugin.workspace_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_logprobs_of_one_token_at_any_stride(dtype):
+    """[N, 1]: contiguous whatever the stride of the dimension of one."""
+    logits, tokens, _ = _case(9, 1, dtype, 3, False)
+    tokens[4] = 1
+    row = logits.flatten().as_strided((9, 1), (1, 9))
+    assert row.is_contiguous() and row.stride(1) != 1
+    _check(scoring.token_logprobs(row, tokens, 2), logits, tokens, 2, None)
+    wide = torch.full((9, 7), torch.nan, device="cuda").to(dtype)
+    wide[:, 3:4] = logits
+    _check(scoring.token_logprobs(wide[:, 3:4], tokens, 2), logits, tokens, 2, None)
+    with pytest.raises(ValueError, match="rows apart"):
+        scoring.token_logprobs(logits[:1].expand(9, 1), tokens)

@@ -68,7 +68,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0,
     if logits.device != dev:
         raise ValueError(f"{what}: tensors on different devices ({logits.device}, {dev})")
     if logits.dim() == 2 and logits.shape[0] > 1:
-        if logits.stride(1) != 1 or logits.stride(0) < vocab:
+        if (logits.stride(1) != 1 and vocab > 1) or logits.stride(0) < vocab:
             raise ValueError(f"{what}: the tokens of a row of logits must be adjacent, its rows apart (strides "
                              f"{logits.stride()})")
         stride = logits.stride(0)
