@@ -344,7 +344,8 @@ int wt_kv8_self_attn(int dtype, const void *qkv, void *k8, void *v8, float *k_sc
  * wt_score_tokens: from hidden states x [N, d] and the projection w [V, d] (fp16 / bf16, d a multiple of 8); the logits
  *   of wt_logits32, never stored. `err`: a device int (zero it once), non-zero after a bounded wait gave up. Needs a
  *   workspace of wt_score_tokens_workspace() bytes (any contents; it depends on the device's SM count; at most some 330
- *   MB: further rows go in passes over it), not shared by calls that may overlap. V <= 2^20, N <= 2^24.
+ *   MB: further rows go in passes over it; 0 for sizes that are refused), not shared by calls that may overlap. V <=
+ *   2^20, N <= 2^24.
  * ------------------------------------------------------------------------------------------------------- */
 int wt_token_logprobs(int dtype, const void *logits, long long row_stride, const int64_t *tokens,
                       const uint8_t *suppress, float *logprob, float *entropy, float *top_logprob, int64_t *top_token,

@@ -43,6 +43,7 @@ constexpr int kSlStageBytes = 2 * kSlABytes;  // x block, then the CTA's half of
 constexpr int kSlSmem = 1024 + kSlStages * kSlStageBytes + (2 * kSlStages + 5) * 8 + 16;
 constexpr int kSlTmem = 512;
 constexpr int kSlErrTimeout = 1;
+constexpr int kSlMaxVocab = 1 << 20, kSlMaxRows = 1 << 24;
 
 // ---- pairs of CTAs -----------------------------------------------------------------------------------------
 __device__ __forceinline__ uint32_t in_first_cta(const void *p) {  // the same place in the pair's first CTA
@@ -598,7 +599,8 @@ int score_rows(int dtype, const uint16_t *x, const void *w, int d, const SlArgs 
 
 extern "C" size_t wt_score_tokens_workspace(int rows, int vocab, int d_model, int top) {
   using namespace wt;
-  if (rows <= 0 || vocab <= 0 || d_model <= 0 || top < 0 || top > kMaxTop) return 0;
+  if (rows <= 0 || vocab <= 0 || d_model <= 0 || top < 0 || top > kMaxTop || vocab > kSlMaxVocab || rows > kSlMaxRows)
+    return 0;
   const int sms = device_sm_count();
   SlPlan p;
   const int take = sl_pass_rows(rows, vocab, d_model, top, sms > 0 ? sms : 148, &p);
@@ -619,7 +621,7 @@ extern "C" int wt_score_tokens(int dtype, const void *x, const void *w, const in
   WT_ALIGNED(w);
   WT_ALIGNED(workspace);
   WT_REQUIRE(d_model % 8 == 0, WT_ERR_UNSUPPORTED, "score_tokens: d_model %d is not a multiple of 8", d_model);
-  WT_REQUIRE(vocab <= (1 << 20) && rows <= (1 << 24), WT_ERR_UNSUPPORTED,
+  WT_REQUIRE(vocab <= kSlMaxVocab && rows <= kSlMaxRows, WT_ERR_UNSUPPORTED,
              "score_tokens: too large (rows %d, vocab %d)", rows, vocab);
   WT_REQUIRE(dtype == WT_F16 || dtype == WT_BF16, WT_ERR_DTYPE, "score_tokens: unknown dtype %d", dtype);
   const int sms = device_sm_count();
