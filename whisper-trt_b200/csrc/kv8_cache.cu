@@ -181,8 +181,6 @@ int launch_append(const void *qkv, const int64_t *offset, void *k8, void *v8, fl
 
 int kv8_append(int dtype, const void *qkv, const int64_t *offset, void *k8, void *v8, float *ks, float *vs, int rows,
                int new_tokens, int heads, int capacity, void *stream) {
-  const long long total = static_cast<long long>(rows) * new_tokens * heads * 2;
-  WT_REQUIRE(total < (1LL << 31), WT_ERR_ARG, "kv8_self_attn: too many new tokens (%d rows x %d)", rows, new_tokens);
   if (dtype == WT_BF16)
     return launch_append<__nv_bfloat16>(qkv, offset, k8, v8, ks, vs, rows, new_tokens, heads, capacity, stream);
   return launch_append<__half>(qkv, offset, k8, v8, ks, vs, rows, new_tokens, heads, capacity, stream);

@@ -307,6 +307,8 @@ extern "C" int wt_kv8_self_attn(int dtype, const void *qkv, void *k8, void *v8, 
              new_tokens);
   WT_REQUIRE(static_cast<unsigned long long>(rows) * heads * capacity < (1ULL << 32), WT_ERR_ARG,
              "kv8_self_attn: the cache has 2^32 slots or more (rows %d x heads %d x %d)", rows, heads, capacity);
+  WT_REQUIRE(!write_cache || static_cast<long long>(rows) * heads * new_tokens * 2 < (1LL << 31), WT_ERR_ARG,
+             "kv8_self_attn: too many new tokens to append (%d rows x heads %d x %d)", rows, heads, new_tokens);
   const int sms = device_sm_count();
   if (sms <= 0) return WT_ERR_CUDA;
   int st;

@@ -15,7 +15,7 @@ inline long long kv8_cross_tiles(int queries) { return (static_cast<long long>(q
 int kv8_cross_tile(int dtype, const void *q, const void *k8, const void *v8, const float *ks, const float *vs,
                    const int64_t *lengths, void *y, int windows, int queries, int heads, int frames, int sms,
                    int *err, void *stream);
-// The new tokens' keys and values into the cache at offset, offset + 1, ... (kv8_cache.cu).
+// The new tokens' keys and values into the cache at offset, offset + 1, ... (kv8_cache.cu); 2 rows heads new_tokens < 2^31.
 int kv8_append(int dtype, const void *qkv, const int64_t *offset, void *k8, void *v8, float *ks, float *vs, int rows,
                int new_tokens, int heads, int capacity, void *stream);
 
