@@ -319,7 +319,8 @@ int wt_linear_residual(int dtype, const void *x, const void *w, const void *b, c
  * wt_kv8_self_attn: qkv [N, S, 3*H*D], y [N, S, H*D]: over the row's slots < offset[r] (clamped to [0, C]), slot j
  *   read from row src[r, j] (clamped to [0, N-1]), and causally over the S new tokens at 16 bits; write_cache != 0:
  *   afterwards (a second kernel: the attention sees the cache as it was) the new keys / values into the row's own slots
- *   offset[r] + s < C. A new token's values that are not finite reach no query before it.
+ *   offset[r] + s < C. A new token's values that are not finite reach no query before it. y must not overlap qkv (that of
+ *   the cross-attention may be q).
  *   Pointers 16-byte aligned, except k_scale, v_scale, lengths, offset and src (their type's alignment).
  * ------------------------------------------------------------------------------------------------------- */
 int wt_kv8_quantize_cross(int dtype, const void *k, const void *v, const int64_t *lengths, void *k8, void *v8,

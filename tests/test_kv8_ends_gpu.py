@@ -181,3 +181,16 @@ def test_cross_queries_past_2_21(s):
     y = kv8.cross_attn(q, cache)
     pick = torch.tensor([0, 1, s // 2, s - 129, s - 2, s - 1], device="cuda")
     _check(y[:, pick], *_cross_reference(q[:, pick], cache, None), 2.0**-20)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("w,s,t", [(3, 5, 100), (1, 5, 1500), (1, 20, 1500), (3, 130, 300), (1, 223, 1500)])
+def test_cross_in_place(dtype, w, s, t):
+    """The result over the queries: every query is read before its result is written, by clusters too."""
+    g = _gen(s)
+    cache = kv8.quantize_cross(_randn(g, w, 4, t, 64, dtype=dtype), _randn(g, w, 4, t, 64, dtype=dtype))
+    q = _randn(g, w, s, 256, dtype=dtype)
+    want = kv8.cross_attn(q, cache)
+    for _ in range(5):
+        y = q.clone()
+        assert kv8.cross_attn(y, cache, out=y) is y and torch.equal(y, want)

@@ -73,6 +73,12 @@ def _check_cache(what: str, cache: Cache8, frames_per_scale: int) -> tuple[int, 
     return r, h, c
 
 
+def _check_apart(what: str, out: torch.Tensor, x: torch.Tensor) -> None:
+    a, b = out.data_ptr(), x.data_ptr()
+    if a < b + x.nbytes and b < a + out.nbytes:
+        raise ValueError(f"{what}: out must not overlap the input")
+
+
 def _check_lengths(what: str, lengths: torch.Tensor | None, windows: int) -> tuple:
     if lengths is None:
         return ()
@@ -115,7 +121,7 @@ def cross_attn(q: torch.Tensor, cache: Cache8, lengths: torch.Tensor | None = No
     """Attention of q [W, S, H*64] to the 8-bit cross cache of T frames -> [W, S, H*64] in q's dtype: the attention of
     :func:`attn_plugin.cross_attn_triton` to the values the cache stands for. ``lengths`` [W] int64: a window attends to
     its first ``lengths[w]`` frames (clamped to [0, T]); what lies behind them is not read, and a window without
-    frames gives zeros."""
+    frames gives zeros (a query whose scores are all -inf gives NaN, as its softmax does). ``out`` may be q itself."""
     what = "kv8.cross_attn"
     w, h, t = _check_cache(what, cache, FRAME_BLOCK)
     shape = q.shape
@@ -132,6 +138,8 @@ def cross_attn(q: torch.Tensor, cache: Cache8, lengths: torch.Tensor | None = No
         y = out
         if y.shape != shape or y.dtype != q.dtype:
             raise ValueError(f"{what}: out must be shaped and typed like q")
+        if y.data_ptr() != q.data_ptr():
+            _check_apart(what, y, q)
         dev = _cuda(what, q, y, *cache, *more)
     if w * s * h == 0:
         return y
@@ -156,7 +164,8 @@ def self_attn(qkv: torch.Tensor, cache: Cache8, offset: torch.Tensor, src: torch
     holds, values that are not finite included, does not reach a query.
 
     ``write_cache``: afterwards the new keys and values go, in 8 bits, into the row's own slots offset, offset + 1, ...
-    (those below C) in place. The attention sees the cache as it was before the call, whatever the slot table names."""
+    (those below C) in place. The attention sees the cache as it was before the call, whatever the slot table names.
+    ``out`` must not overlap qkv: other rows' tokens are read, and appended, while it is written."""
     what = "kv8.self_attn"
     n, h, c = _check_cache(what, cache, 1)
     shape = qkv.shape
@@ -176,6 +185,7 @@ def self_attn(qkv: torch.Tensor, cache: Cache8, offset: torch.Tensor, src: torch
         y = out
         if y.shape != (n, s, h * HEAD_DIM) or y.dtype != qkv.dtype:
             raise ValueError(f"{what}: out must be [N, S, H*64] of qkv's dtype")
+        _check_apart(what, y, qkv)
         dev = _cuda(what, qkv, y, *cache, offset, src)
     if n * s * h == 0:
         return y
