@@ -20,12 +20,12 @@ which makes the error word of the device's waits). CUDA tensors only, contiguous
 
 from __future__ import annotations
 
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .attn_plugin import _cuda, _dtype_code, _on, _stream, _workspace
+from .attn_plugin import NAMESPACE, _cuda, _dtype_code, _on, _stream, _workspace
 
 HEAD_DIM = 64
 FRAME_BLOCK = 64  # frames of a cross-attention cache that share a scale
@@ -198,3 +198,63 @@ def self_attn(qkv: torch.Tensor, cache: Cache8, offset: torch.Tensor, src: torch
                                           _stream(dev))
     _lib.check(st, what)
     return y
+
+
+# --- torch custom ops (for tracing: fake kernels, and what a call writes declared) --------------------------
+@torch.library.custom_op(f"{NAMESPACE}::kv8_quantize_cross", mutates_args=())
+def quantize_cross_op(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor]
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`quantize_cross` into a new cache, whose four tensors it returns."""
+    return tuple(quantize_cross(k, v, lengths))
+
+
+@quantize_cross_op.register_fake
+def _(k, v, lengths):
+    w, h, t, _ = k.shape
+    blocks = (t + FRAME_BLOCK - 1) // FRAME_BLOCK
+    return (*(k.new_empty(k.shape, dtype=torch.float8_e4m3fn) for _ in range(2)),
+            *(k.new_empty(w, h, blocks, dtype=torch.float32) for _ in range(2)))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_quantize_cross_into", mutates_args=("k8", "v8", "k_scale", "v_scale"))
+def quantize_cross_into_op(k: torch.Tensor, v: torch.Tensor, lengths: Optional[torch.Tensor], k8: torch.Tensor,
+                           v8: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> None:
+    """:func:`quantize_cross` into the cache of the last four."""
+    quantize_cross(k, v, lengths, out=Cache8(k8, v8, k_scale, v_scale))
+
+
+@quantize_cross_into_op.register_fake
+def _(k, v, lengths, k8, v8, k_scale, v_scale):
+    return None
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_cross_attn", mutates_args=())
+def cross_attn_op(q: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                  lengths: Optional[torch.Tensor]) -> torch.Tensor:
+    """:func:`cross_attn`."""
+    return cross_attn(q, Cache8(k8, v8, k_scale, v_scale), lengths)
+
+
+@cross_attn_op.register_fake
+def _(q, k8, v8, k_scale, v_scale, lengths):
+    return torch.empty_like(q)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_self_attn", mutates_args=())
+def self_attn_op(qkv: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                 offset: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
+    """:func:`self_attn` without the append."""
+    return self_attn(qkv, Cache8(k8, v8, k_scale, v_scale), offset, src)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::kv8_self_attn_append", mutates_args=("k8", "v8", "k_scale", "v_scale"))
+def self_attn_append_op(qkv: torch.Tensor, k8: torch.Tensor, v8: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, offset: torch.Tensor, src: torch.Tensor) -> torch.Tensor:
+    """:func:`self_attn` that appends the new keys and values at ``offset``."""
+    return self_attn(qkv, Cache8(k8, v8, k_scale, v_scale), offset, src, write_cache=True)
+
+
+@self_attn_op.register_fake
+@self_attn_append_op.register_fake
+def _(qkv, k8, v8, k_scale, v_scale, offset, src):
+    return qkv.new_empty(qkv.shape[0], qkv.shape[1], k8.shape[1] * HEAD_DIM)

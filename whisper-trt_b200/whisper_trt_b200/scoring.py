@@ -18,12 +18,12 @@ such token has entropy 0 and log-probability -inf. A NaN or +inf logit makes a r
 
 from __future__ import annotations
 
-from typing import NamedTuple
+from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .attn_plugin import _cuda, _dtype_code, _on, _stream, _workspace
+from .attn_plugin import NAMESPACE, _cuda, _dtype_code, _on, _stream, _workspace
 
 MAX_TOP = 16
 
@@ -119,3 +119,35 @@ def score_tokens(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, top: in
                                  scratch.data_ptr(), nbytes, _stream(dev))
     _lib.check(st, what)
     return out
+
+
+# --- torch custom ops (for tracing) -------------------------------------------------------------------------
+def _fake(tokens: torch.Tensor, top: int):
+    lead = tokens.shape
+    f32 = torch.float32
+    return (tokens.new_empty(lead, dtype=f32), tokens.new_empty(lead, dtype=f32),
+            tokens.new_empty((*lead, top), dtype=f32), tokens.new_empty((*lead, top)))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::token_logprobs", mutates_args=())
+def token_logprobs_op(logits: torch.Tensor, tokens: torch.Tensor, top: int, suppress: Optional[torch.Tensor]
+                      ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`token_logprobs`: logprob, entropy, top_logprob, top_token."""
+    return tuple(token_logprobs(logits, tokens, top, suppress))
+
+
+@token_logprobs_op.register_fake
+def _(logits, tokens, top, suppress):
+    return _fake(tokens, top)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::score_tokens", mutates_args=())
+def score_tokens_op(x: torch.Tensor, w: torch.Tensor, tokens: torch.Tensor, top: int, suppress: Optional[torch.Tensor]
+                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """:func:`score_tokens`, likewise."""
+    return tuple(score_tokens(x, w, tokens, top, suppress))
+
+
+@score_tokens_op.register_fake
+def _(x, w, tokens, top, suppress):
+    return _fake(tokens, top)
