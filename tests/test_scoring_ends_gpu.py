@@ -61,3 +61,27 @@ def test_logprobs_of_one_token_at_any_stride(dtype):
     _check(scoring.token_logprobs(wide[:, 3:4], tokens, 2), logits, tokens, 2, None)
     with pytest.raises(ValueError, match="rows apart"):
         scoring.token_logprobs(logits[:1].expand(9, 1), tokens)
+
+
+@pytest.mark.parametrize("suppress", [False, True])
+@pytest.mark.parametrize("n,v", [(3, 2**20), (5, 2**20 - 7), (300, 2**20 - 1)])
+def test_vocabularies_near_2_20(n, v, suppress):
+    """The largest masks, and more records a row than a CTA of the merge takes at once."""
+    logits, tokens, sup = _case(n, v, torch.bfloat16, n, suppress)
+    tokens[0] = v - 1
+    _check(scoring.token_logprobs(logits, tokens, 16, sup), logits, tokens, 16, sup)
+    x, w, tokens, sup = _states(n, v, 64, torch.float16, n, suppress)
+    tokens[0] = v - 1
+    got = scoring.score_tokens(x, w, tokens, 16, sup)
+    for a in range(0, n, 50):
+        part = slice(a, a + 50)
+        _check(scoring.TokenScores(*(y[part] for y in got)), x[part].double() @ w.double().t(), tokens[part], 16, sup)
+    assert attn_plugin.workspace_errors() == 0
+
+
+def test_vocabularies_past_2_20_are_refused():
+    with pytest.raises(ValueError):
+        scoring.token_logprobs(torch.zeros(1, 2**20 + 1, device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda"))
+    with pytest.raises(ValueError, match="too large"):
+        scoring.score_tokens(torch.zeros(1, 8, device="cuda").half(), torch.zeros(2**20 + 1, 8, device="cuda").half(),
+                             torch.zeros(1, dtype=torch.int64, device="cuda"))
