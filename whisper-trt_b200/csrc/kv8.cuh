@@ -79,6 +79,11 @@ __device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t x) {
   return r;
 }
 
+// 8 e4m3 values as fp16.
+__device__ __forceinline__ uint4 widen_f16(uint32_t a, uint32_t b) {
+  return make_uint4(e4m3_to_f16x2(a), e4m3_to_f16x2(a >> 16), e4m3_to_f16x2(b), e4m3_to_f16x2(b >> 16));
+}
+
 __device__ __forceinline__ float ex2f(float x) {  // 2^x on the special-function unit (2^-inf = 0)
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -26,10 +26,6 @@ namespace {
 constexpr int kTQ = 64, kTK = 64, kTThreads = 128;
 constexpr int kTTile = 64 * 128;  // 64 rows of 128 bytes
 
-// One 8-byte half of a 16-byte e4m3 piece as 16 bytes of 16-bit values.
-__device__ __forceinline__ uint4 widen_f16(uint32_t a, uint32_t b) {
-  return make_uint4(e4m3_to_f16x2(a), e4m3_to_f16x2(a >> 16), e4m3_to_f16x2(b), e4m3_to_f16x2(b >> 16));
-}
 __device__ __forceinline__ uint32_t f16x2_to_bf16x2(uint32_t h) {
   const float2 f = Elem<__half>::to_float2(h);
   return Elem<__nv_bfloat16>::from_float2(f.x, f.y);

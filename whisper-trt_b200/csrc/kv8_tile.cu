@@ -68,9 +68,6 @@ constexpr int kTKv = kTQTile, kTSlotsAt = kTKv + kTStages * 2 * kTKTile, kTBars 
 static_assert(kTQ * kTRec * 4 <= kTStages * 2 * kTKTile, "a CTA's share lies over the tiles");
 static_assert(2 * (kTBytes + 5 * 1024) <= 228 * 1024, "two CTAs on an SM (static arrays and the reserved 1 KB with them)");
 
-__device__ __forceinline__ uint4 widen_f16(uint32_t a, uint32_t b) {  // 8 e4m3 bytes
-  return make_uint4(e4m3_to_f16x2(a), e4m3_to_f16x2(a >> 16), e4m3_to_f16x2(b), e4m3_to_f16x2(b >> 16));
-}
 // Tensor memory of 16 rows by 64 or 16 columns, as an MMA's accumulator lies in registers: of each 8 columns a lane holds
 // columns 2 (lane % 4) and + 1 of rows lane / 4 (r[4 i], r[4 i + 1]) and + 8 (r[4 i + 2], r[4 i + 3]).
 __device__ __forceinline__ void tmem_ld_rows64(uint32_t taddr, uint32_t (&r)[32]) {
