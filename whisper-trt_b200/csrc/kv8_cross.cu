@@ -311,9 +311,9 @@ int cross8(const void *q, const void *k8, const void *v8, const float *ks, const
   // 4 x 4 (3 CTAs) 7.9 / 11.0 / 17.2 / 26.8 / 44.9; 2 x 4 6.5 / 12.8 / 21.5 / 29.1 / 47.2; 8 x 2 11.0 / 12.9 / 16.7 /
   // 26.3 / 44.8.
   if (nt == 1) return launch_cross8<T, 1, 4, 2>(q, k8, v8, ks, vs, lengths, y, W, S, H, Tn, cl, stream);
-  // More queries take more registers: 9 to 24 run with 3 CTAs on an SM. Measured (us at 32 windows, fp16 / bf16): 16
-  // queries 35.0 / 31.3, in as many registers as they like (2 CTAs, rings of 4 units) 42.6 / 39.5, 4 CTAs 37.5 / 33.6; 24
-  // queries 48.6 / 43.0, with 2 CTAs 53.2 / 48.5, as 4 tiles 66.6 / 61.2; 32 queries 67.0 / 60.8, with 3 CTAs 68.4 / 62.8.
+  // More queries take more registers: 9 to 24 run with 3 CTAs on an SM. Measured (us at 32 windows, fp16): 16 queries 34.7, in as
+  // many registers as they like (2 CTAs, rings of 4 units) 42.6, 4 CTAs 37.5; 24 queries 48.7, with 2 CTAs 53.2, as 4 tiles
+  // 66.6; 32 queries 67.4, with 3 CTAs 68.4. In bf16, whose queries are scaled first, 35.5, 51.0 and 70.3.
   if (nt == 2) return launch_cross8<T, 2, 4, 2>(q, k8, v8, ks, vs, lengths, y, W, S, H, Tn, cl, stream);
   if (nt == 3) return launch_cross8<T, 3, 4, 2>(q, k8, v8, ks, vs, lengths, y, W, S, H, Tn, cl, stream);
   return launch_cross8<T, 4, 4, 3>(q, k8, v8, ks, vs, lengths, y, W, S, H, Tn, cl, stream);
@@ -343,8 +343,9 @@ extern "C" int wt_kv8_cross_attn(int dtype, const void *q, const void *k8, const
   const int sms = device_sm_count();
   if (sms <= 0) return WT_ERR_CUDA;
   // Up to 32 queries share one read of the keys here, and the tile kernel's 128 rows would be mostly empty. Measured (us, here
-  // / tile kernel, 20 heads x 1500 frames, fp16): 1 window x 32 queries 11.5 / 12.8, x 33 13.1 / 12.8, x 128 24.0 / 15.5; 4
-  // windows x 33 26.6 / 24.6; 16 windows x 32 43.4 / 58, x 64 67.4 / 58.
+  // / tile kernel, 20 heads x 1500 frames, fp16): 1 window x 32 queries 11.2 / 11.9; 16 windows x 32 43.7 / 56.8, of which it
+  // takes 64 in 57.4. (A second round of 32 queries here took 13.1 at 1 window x 33, the tile kernel 12.2; 26.6 / 23.3 at 4
+  // windows.)
   if (queries > 32)
     return kv8_cross_tile(dtype, q, k8, v8, k_scale, v_scale, lengths, y, windows, queries, heads, frames, sms, err,
                           stream);

@@ -4,8 +4,8 @@
 // One CTA of 4 warps per 64 queries of a (row, head): queries are the M of mma.sync.m16n8k16 (16 a warp), keys the N, in
 // blocks of 64; the longest CTAs come first. A row's keys are few (a prompt and what stands before it), so a CTA lives
 // for a handful of blocks, and its start and the exchange between its warps count for as much as its products: on tcgen05
-// (kv8_tile.cu's kernel then, M 128, with the new tokens as further blocks) 32 rows x 223 tokens x 20 heads took 79 us,
-// here 58 (memory alone: 9). Bound by latency: 4 CTAs on an SM in 128 registers, a few of them spilled; 3 CTAs in 168
+// (a form of kv8_tile.cu's kernel with a softmax thread a query and the weights through shared memory, M 128, the new tokens
+// as further blocks; the present form was not tried) 32 rows x 223 tokens x 20 heads took 79 us, here 58 (memory alone: 9). Bound by latency: 4 CTAs on an SM in 128 registers, a few of them spilled; 3 CTAs in 168
 // took 64, 32 keys at a time 63 (4 CTAs) and 73 (5).
 // With many queries a key serves the whole CTA, so a block is converted once, on its way into shared memory: the next
 // block's e4m3 bytes (and slot-table entries, a block earlier still) are loaded into registers while the current one is

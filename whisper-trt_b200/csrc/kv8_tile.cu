@@ -7,16 +7,17 @@
 //   * warps 0-7 are the softmax, 16 queries each, 4 lanes a query, in the layout of an MMA's accumulator: maxima and sums
 //     cross lanes in two shuffles, and the weights go, as 16-bit pairs, over the scores they come from, from where the
 //     second product takes them (no trip through shared memory: with it and a thread a query the 16 windows below took 51
-//     us). They are relative to a maximum that lags: only when a score exceeds it by 2^kLag does the warp take the output
-//     out of tensor memory and rescale it, which is rare after the first block.
+//     us instead of 43, weights then in one part). They are relative to a maximum that lags: only when a score exceeds it
+//     by 2^kLag does the warp take the output out of tensor memory and rescale it, which is rare after the first block.
 //   * warps 8-11 bring a block in: e4m3 bytes by asynchronous copies three ahead, converted once for all queries -- exactly,
 //     to fp16 -- and stored as they lie, 64 rows of 128 swizzled bytes: K's is the product's K-major operand, V's its
-//     MN-major one (transposing V on the way took 47 us instead of 43).
+//     MN-major one (transposing V on the way took 47 us instead of 43, likewise).
 //   * warp 12 issues the MMAs: the next two blocks' S before it waits for a block's weights.
 // Windows of different lengths go longest first, so that no long one is left to the end on its own: every CTA reads the
 // lengths and counts its window's place (57 -> 51 us). Where there are too few tiles of queries for the SMs, a cluster of 2 or
 // 4 CTAs shares a tile's frames; their sums meet through distributed shared memory.
-// 16 windows x 223 queries x 16 heads, lengths 375 to 1500, bf16: 43 us; memory alone 8, exponentials (16 a cycle) 14.
+// 16 windows x 223 queries x 16 heads, lengths 375 to 1500, bf16: 51 us, of which the weights' second part takes 7; memory
+// alone 8, exponentials (16 a cycle) 14.
 // Bound by hand-offs: a block's way from MMA to softmax to MMA takes some 1000 cycles with nothing to compute, 1300 with it;
 // two CTAs on an SM and three S in flight hide part of it. Fewer copies, one exponential for all, a stage more: 2 to 5%.
 //
@@ -537,8 +538,8 @@ int launch_tile(TileArgs a, int sms, void *stream) {
   a.tiles = static_cast<int>(kv8_cross_tiles(a.S));
   const long long units = static_cast<long long>(a.W) * a.H * a.tiles;  // (fewer than 2^30)
   // CTAs per tile of queries, a cluster that shares its frames: as many as two on each SM hold, of 3 blocks at least. Measured
-  // (us, 20 heads x 1500 frames, fp16, with / without): 1 window x 64 queries 14.5 / 25.8, x 223 20.5 / 26.3, x 448 26.7 /
-  // 33; 2 windows x 128 21.0 / 26.2; 4 windows x 64, one more per SM than without, 25.9 / 26.5.
+  // (us, 20 heads x 1500 frames, fp16, with / without): 1 window x 33 queries 12.2 / 25.0, x 128 14.0 / 25.5, x 223 19.3 / 25.7;
+  // 2 windows x 128 19.3 / 25.6; 4 windows x 64, which take every second place of the SMs' already, 24.6 / 25.9.
   a.cl = 1;
   while (a.cl < kTCluster && units * a.cl * 2 <= 2LL * sms && a.T > a.cl * 2 * 3 * kTK) a.cl *= 2;
   constexpr int smem = kTBytes;

@@ -588,7 +588,7 @@ int score_rows(int dtype, const uint16_t *x, const void *w, int d, const SlArgs 
 #undef WT_SCORE_CASE
   if (st != WT_OK) return st;
   // (with 5 alternatives of 51866 tokens, us of the whole call by a warp / a CTA a row: 160 rows x 136 records 48.9 / 44.5,
-  // 512 x 74 82.2 / 82.1, 1024 x 36 124 / 134, 7136 x 58 829 / 864)
+  // 512 x 74 82.2 / 82.1, 1024 x 36 124 / 134, 7136 x 58 770 to 829 by the power cap / 864)
   if (a.p.parts <= 64)
     return launch("score_tokens", score_merge_kernel, dim3((a.N + 3) / 4), dim3(128), 0, stream, a, out);
   return launch("score_tokens", score_merge_wide_kernel, dim3(a.N), dim3(256), 0, stream, a, out);
